@@ -112,7 +112,8 @@ int gemq_version(void);
  * The first error recorded since the last call: 1-7 a bounded wait of the GEMM
  * pipeline expired (copies landed, stage freed, A stage written, A stage read,
  * accumulator full, accumulator free, drain), 8 an expert id out of range, 9 a
- * bit-width outside 1..4, 10 a KV-cache position past the cache, 11 a chained
+ * bit-width outside 1..4, 10 a KV-cache position, length or page id outside the
+ * cache, 11 a chained
  * down-projection item waited too long for its gate/up tiles. After an expired wait
  * the kernels of that forward drain and return; its outputs are undefined. */
 int gemq_get_device_error(uint32_t* code_out /* host */);
@@ -342,6 +343,116 @@ int gemq_qk_norm_rope(const uint16_t* qkv, int64_t ld, int64_t rows, int32_t n, 
 int gemq_decode_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, int32_t heads,
                           int32_t max_len, int32_t head_dim, const int64_t* cache_len, float scale, uint16_t* out,
                           void* stream);
+
+/* ---------------------------------------------------------------- serving: paged KV cache
+ * No counterpart in the reference, whose generate loop keeps one sequence's fp16 cache
+ * (gemq/benchmark_generate.py:113-156): a cache of pages that several sequences share,
+ * attention over it, and the verification of drafted tokens. */
+#define GEMQ_FP16 0
+#define GEMQ_BF16 1
+#define GEMQ_FP32 2
+
+/*
+ * One layer's cache. Rows of head_dim elements, one per page, KV head and token of the
+ * page; a row is contiguous, the strides between pages, heads and tokens are free (k and
+ * v share them). A slot is page * page_size + token of the page.
+ *   bits 16: values of `dtype`; no scales.
+ *   bits 8:  int8 codes; scales [step]: value = code * step.
+ *   bits 4:  two codes to a byte, the even element in the low half; scales [step, base]:
+ *            value = code * step + base.
+ * Limits: head_dim a multiple of 16, at most 256; page_size a power of two, at most
+ * 65536; num_pages * page_size below 2^31; k, v and the code strides multiples of 16
+ * bytes (8 for bits 4 with head_dim % 32 != 0); scales 4-byte (bits 8) or 8-byte (bits 4)
+ * aligned.
+ */
+typedef struct gemq_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;            /* NULL for bits 16 */
+  float* v_scale;
+  int64_t strides[3];        /* codes: bytes between pages, heads, tokens */
+  int64_t scale_strides[3];  /* scales: floats between pages, heads, tokens */
+  int32_t num_pages;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+  int32_t bits;              /* 16, 8 or 4 */
+  int32_t dtype;             /* GEMQ_FP16 or GEMQ_BF16: rows written and read, queries, outputs */
+} gemq_kv_cache_t;
+
+/* Writes token t's keys and values k, v [tokens, kv_heads, head_dim] (strides in elements
+ * between tokens and heads; rows 16-byte aligned) to slot slots[t]. A negative slot skips
+ * its token, one past the cache is recorded in the device error word and skipped; of two
+ * tokens with one slot either may stay. Per row x: 8 bits m = max(max|x|, 127 * 2^-64),
+ * code rint(127 x / m), step m / 127; 4 bits lo = min x, r = max(max x - lo, 15 * 2^-64),
+ * code rint(15 (x - lo) / r), step r / 15, base lo. A row with a NaN, an infinity or a
+ * product above that leaves fp32 reads back as NaN throughout. */
+int gemq_kv_cache_write(const gemq_kv_cache_t* cache /* host */, const void* k, const void* v, int64_t k_token_stride,
+                        int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                        int64_t tokens, void* stream);
+
+/* Reads slots[t] back: k_out, v_out [tokens, kv_heads, head_dim] of the cache's dtype,
+ * contiguous, 16-byte aligned; zeros for a negative slot or one past the cache. */
+int gemq_kv_cache_read(const gemq_kv_cache_t* cache /* host */, const int64_t* slots, int64_t tokens, void* k_out,
+                       void* v_out, void* stream);
+
+/* Attention of new tokens over the cache, which already holds their own keys and values.
+ * Sequence b has the tokens [q_starts[b], q_starts[b + 1]) of q (q_starts NULL:
+ * num_tokens / num_seqs each) and kv_lens[b] positions with them; position j lies in page
+ * page_table[b * page_table_stride + j / page_size]. Token i of n sees the positions
+ * j <= kv_lens[b] - n + i, and with window > 0 only the last `window` of those; a row
+ * that sees nothing gives zeros and lse -inf, and what a row does not see does not reach
+ * it, whatever it holds. q_heads is a multiple of kv_heads; head h reads KV head
+ * h / (q_heads / kv_heads). q [num_tokens, q_heads, head_dim] (token stride in elements,
+ * a multiple of 8; 16-byte aligned); out the same, contiguous; lse fp32 [num_tokens,
+ * q_heads] or NULL: the natural logarithm of the sum of exp(scale * score). Scores,
+ * softmax statistics and sums are fp32. Tokens outside every sequence are not written.
+ * max_q_len and max_kv_len (0: unknown) are the longest values the call may meet; they
+ * choose the kernel and the split, and longer ones stay right. Lengths, starts and page
+ * ids outside the buffers are clamped or skipped and recorded in the device error word. */
+size_t gemq_paged_attention_workspace_size(const gemq_kv_cache_t* cache /* host */, int64_t num_tokens,
+                                           int32_t q_heads, int32_t num_seqs, int32_t max_pages, int32_t max_q_len,
+                                           int32_t max_kv_len);
+int gemq_paged_attention(const gemq_kv_cache_t* cache /* host */, const void* q, int64_t q_token_stride,
+                         int64_t num_tokens, int32_t q_heads, const int32_t* page_table, int64_t page_table_stride,
+                         int32_t max_pages, const int32_t* kv_lens, const int32_t* q_starts, int32_t num_seqs,
+                         int32_t max_q_len, int32_t max_kv_len, float scale, int32_t window, void* out, float* lse,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Verification of drafted tokens. p_i = softmax(logits[b][i] / temperature[b]) (NULL: 1;
+ * 0: all of it on the first maximum); draft i < draft_lens[b] (NULL: num_drafts) is taken
+ * while uniforms[b][i] * q_i(x_i) < p_i(x_i), with q_i = draft_probs[b][i] (NULL: the
+ * draft was certain, q_i(x_i) = 1). At the first position r that is not taken, or at the
+ * draft's end, one token is drawn from w = max(p_r - q_r, 0) (at the end, or where that
+ * leaves nothing, w = p_r): the j with the largest w_j / noise[b][j], lowest j on ties;
+ * exponential noise makes that a sample of w / sum(w).
+ * tokens int64 [B, n + 1]: the taken drafts, the drawn token, then -1; num_accepted int32
+ * [B]; logprobs fp32 [B, n + 1]: log softmax(logits / T) of each token (T = 1 where the
+ * temperature is 0), 0 beside a -1. A row with a NaN, a +inf or nothing finite, or a
+ * temperature below zero or NaN, has no distribution: its draft is not taken and the
+ * token drawn there is -1. A draft outside the vocabulary is not taken.
+ * 1 <= num_drafts <= 63, num_seqs <= 65535, vocab < 2^30. */
+typedef struct gemq_verify {
+  const void* logits;         /* [num_seqs][num_drafts + 1][vocab] */
+  int64_t logits_seq_stride;  /* elements */
+  int64_t logits_row_stride;
+  int32_t logits_dtype;       /* GEMQ_FP16, GEMQ_BF16 or GEMQ_FP32 */
+  int32_t probs_dtype;
+  const int64_t* draft_tokens; /* [num_seqs][num_drafts] */
+  const void* draft_probs;    /* [num_seqs][num_drafts][vocab] or NULL */
+  int64_t probs_seq_stride;
+  int64_t probs_row_stride;
+  const int32_t* draft_lens;  /* [num_seqs] or NULL */
+  const float* uniforms;      /* [num_seqs][num_drafts], in [0, 1) */
+  const float* noise;         /* [num_seqs][vocab], > 0 */
+  const float* temperature;   /* [num_seqs] or NULL */
+  int64_t* tokens;
+  int32_t* num_accepted;
+  float* logprobs;
+} gemq_verify_t;
+size_t gemq_verify_draft_workspace_size(int32_t num_seqs, int32_t num_drafts, int32_t vocab);
+int gemq_verify_draft(const gemq_verify_t* args /* host */, int32_t num_seqs, int32_t num_drafts, int32_t vocab,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -53,6 +53,8 @@ EXPORTED = [
     "gemq_dispatch_workspace_size", "gemq_moe_dispatch", "gemq_moe_experts_workspace_size", "gemq_moe_experts",
     "gemq_moe_experts_row_order", "gemq_layer_dequant_forms", "gemq_rms_norm",
     "gemq_qk_norm_rope", "gemq_decode_attention", "gemq_layer_set_routing", "gemq_route_ex",
+    "gemq_kv_cache_write", "gemq_kv_cache_read", "gemq_paged_attention_workspace_size", "gemq_paged_attention",
+    "gemq_verify_draft_workspace_size", "gemq_verify_draft",
 ]
 
 
@@ -98,6 +100,35 @@ class RoutingT(ctypes.Structure):
     ]
 
 
+# element types of the serving operators
+FP16, BF16, FP32 = 0, 1, 2
+
+
+class KvCacheT(ctypes.Structure):
+    """gemq_kv_cache_t: one layer's paged key/value cache."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("strides", ctypes.c_int64 * 3), ("scale_strides", ctypes.c_int64 * 3),
+        ("num_pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("bits", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class VerifyT(ctypes.Structure):
+    """gemq_verify_t: the tensors of one verification of drafted tokens."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("logits_seq_stride", ctypes.c_int64), ("logits_row_stride", ctypes.c_int64),
+        ("logits_dtype", ctypes.c_int32), ("probs_dtype", ctypes.c_int32),
+        ("draft_tokens", ctypes.c_void_p), ("draft_probs", ctypes.c_void_p),
+        ("probs_seq_stride", ctypes.c_int64), ("probs_row_stride", ctypes.c_int64),
+        ("draft_lens", ctypes.c_void_p), ("uniforms", ctypes.c_void_p), ("noise", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("num_accepted", ctypes.c_void_p),
+        ("logprobs", ctypes.c_void_p),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 _lock = threading.Lock()
 
@@ -139,6 +170,13 @@ def _declare(lib: ctypes.CDLL) -> None:
         "gemq_dispatch_workspace_size": (sz, [i64, i32, i32]),
         "gemq_moe_dispatch": (ctypes.c_int, [vp, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp]),
         "gemq_moe_experts_row_order": (ctypes.c_int, [vp]),
+        "gemq_kv_cache_write": (ctypes.c_int, [P(KvCacheT), vp, vp, i64, i64, i64, i64, vp, i64, vp]),
+        "gemq_kv_cache_read": (ctypes.c_int, [P(KvCacheT), vp, i64, vp, vp, vp]),
+        "gemq_paged_attention_workspace_size": (sz, [P(KvCacheT), i64, i32, i32, i32, i32, i32]),
+        "gemq_paged_attention": (ctypes.c_int, [P(KvCacheT), vp, i64, i64, i32, vp, i64, i32, vp, vp, i32, i32, i32,
+                                                ctypes.c_float, i32, vp, vp, vp, sz, vp]),
+        "gemq_verify_draft_workspace_size": (sz, [i32, i32, i32]),
+        "gemq_verify_draft": (ctypes.c_int, [P(VerifyT), i32, i32, i32, vp, sz, vp]),
         "gemq_moe_experts_workspace_size": (sz, [vp, i64, i32]),
         "gemq_moe_experts": (ctypes.c_int, [vp, vp, i64, vp, i32, vp, vp, i32, u32, vp, sz, vp]),
     }

@@ -1,0 +1,148 @@
+// What the paged KV cache's kernels share: the cache's device description, one row's
+// address, and the 16-bit types.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "gemq_common.cuh"
+#include "gemq_internal.h"
+
+namespace gemq {
+
+// The smallest step a quantised row is stored with. Attention weights each value row by
+// its step (2^log2 step), so the step must not be zero; 2^-64 is far below any real
+// row's (a fp16 row's step is at least 2^-31 unless it is constant) and keeps 1 / step
+// times any sequence length inside fp32.
+constexpr float kMinScale = 5.421010862427522e-20f;  // 2^-64
+
+// gemq_kv_cache_t as the kernels take it. Strides: bytes between pages, heads and
+// tokens of the codes; floats between those of the scales.
+struct KvDev {
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_token_stride;
+  int num_pages, kv_heads, page_shift, head_dim;
+
+  __device__ __forceinline__ int64_t row(int page, int head, int off) const {
+    return page * page_stride + head * head_stride + off * token_stride;
+  }
+  __device__ __forceinline__ int64_t scale_row(int page, int head, int off) const {
+    return page * scale_page_stride + head * scale_head_stride + off * scale_token_stride;
+  }
+};
+
+template <typename T>
+struct Vec2;
+template <>
+struct Vec2<__half> {
+  using type = __half2;
+};
+template <>
+struct Vec2<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two fp32 values rounded to a pair of T, as the 32 bits of the pair.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
+// Everything an attention launch needs.
+struct AttnArgs {
+  KvDev kv;
+  const void* q;
+  int64_t q_token_stride;  // elements
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  int max_pages;
+  const int32_t* kv_lens;
+  const int32_t* q_starts;  // null: every sequence has num_tokens / num_seqs tokens
+  int num_tokens, num_seqs, q_heads, group;
+  float scale;
+  int window;  // 0: none
+  void* out;
+  float* lse;  // may be null
+};
+
+// New tokens [start, start + len) of sequence b and its length with them, clamped to the
+// buffers (a value outside them is recorded in the device error word).
+struct SeqRange {
+  int start, q_len, kv_len;
+};
+__device__ __forceinline__ SeqRange seq_range(const AttnArgs& a, int b) {
+  SeqRange r;
+  int lo, hi;
+  if (a.q_starts != nullptr) {
+    lo = a.q_starts[b];
+    hi = a.q_starts[b + 1];
+  } else {
+    const int n = a.num_tokens / a.num_seqs;
+    lo = b * n;
+    hi = lo + n;
+  }
+  const int kv = a.kv_lens[b];
+  const int cap = a.max_pages << a.kv.page_shift;
+  r.start = min(max(lo, 0), a.num_tokens);
+  r.q_len = min(max(hi, r.start), a.num_tokens) - r.start;
+  r.kv_len = min(max(kv, 0), cap);
+  if (lo != r.start || hi != r.start + r.q_len || kv != r.kv_len) set_device_error(kDevBadCachePos);
+  return r;
+}
+
+// The page of a sequence's page index, or -1 (recorded) for an id outside the cache.
+__device__ __forceinline__ int page_of(const AttnArgs& a, int b, int index) {
+  const int p = a.page_table[b * a.page_table_stride + index];
+  if (p >= 0 && p < a.kv.num_pages) return p;
+  set_device_error(kDevBadCachePos);
+  return -1;
+}
+
+// Launchers (kernels_cache.cu, kernels_attn.cu, kernels_verify.cu). Arguments are checked
+// by the C ABI before they come here.
+cudaError_t launch_cache_write(const KvDev& c, int bits, bool bf16, const void* k, const void* v, int64_t k_ts,
+                               int64_t k_hs, int64_t v_ts, int64_t v_hs, const int64_t* slots, int tokens,
+                               cudaStream_t s);
+cudaError_t launch_cache_read(const KvDev& c, int bits, bool bf16, const int64_t* slots, int tokens, void* k, void* v,
+                              cudaStream_t s);
+size_t attention_workspace(const AttnArgs& a, int bits, int max_q_len, int max_kv_len);
+cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
+                             cudaStream_t s);
+size_t verify_workspace(int B, int n, int V);
+cudaError_t launch_verify(const gemq_verify_t& v, int B, int n, int V, void* workspace, cudaStream_t s);
+
+}  // namespace gemq
