@@ -2,180 +2,868 @@
 //
 // Row (token i of the n new ones of a sequence of length L with them, query head h) has
 // position p = L - n + i and sees the keys j <= p (j > p - window where there is one):
-//   o = sum_j w_j v_j / sum_j w_j,  w_j = 2^(c q.k_j - m),  c = scale log2(e),
+//   o = sum_j w_j v_j / sum_j w_j,  w_j = 2^(x_j - m),  x_j = scale log2(e) q.k_j,
 //   lse = (m + log2 sum_j w_j) ln(2)
 // A row that sees nothing gives o = 0 and lse = -inf. What a row does not see does not
 // reach it whatever it holds.
+//
+// Quantised rows, k_j = s_j c_j (8 bits) or s_j (c_j - 8) + z_j (4 bits, z_j the value of
+// code 8), and the same for v with step t_j and value y_j of code 8, go to the tensor
+// cores as their codes, which are exact in fp16:
+//   q.k_j = s_j (q.c_j) + z_j sum(q)
+//   o = sum_j w'_j (c_j + y_j / t_j) / sum_j w'_j / t_j,  w'_j = 2^(x_j + log2 t_j - m)
+// so the value's step acts as a shift of the score, w' stays in [0, 1], and the only
+// rounding below 32 bits is that of w' to 16 bits, as without quantisation.
+//
+// This file: few rows a KV head (decode steps, drafted tokens), where the cache's bytes
+// are the time. mma.sync with the 16 rows of one KV head (tokens x query heads that share
+// it) as M: at most 1/8 of the legacy tensor rate is needed to keep up with HBM, so the
+// tensor-memory form would only add its round trips. Every warp streams its own tiles of
+// 16 or 32 keys through its own cp.async ring, without block barriers; the keys of all
+// sequences and heads form one axis of 64- or 128-key units that is cut evenly over all
+// blocks (so uneven lengths do not matter), and k_attn_join adds up heads that were cut.
+#include <algorithm>
+
+#include "attn_rows.cuh"
 #include "paged.cuh"
 
 namespace gemq {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+// ------------------------------------------------------------------ small pieces
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Eight elements of a stored row, from element 8 * c.
-template <typename T, int BITS>
-__device__ __forceinline__ void load8(const uint8_t* row, int c, float step, float base, float (&x)[8]) {
-  if constexpr (BITS == 16) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + c * 16);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2<T>(u[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  } else if constexpr (BITS == 8) {
-    const uint2 w = *reinterpret_cast<const uint2*>(row + c * 8);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)))) * step;
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
+  if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
   } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + c * 4);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((w >> (4 * i)) & 15u), step, base);
+    static_assert(N == 4, "two or four words");
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(a)
+                 : "memory");
   }
 }
 
-constexpr int kRowThreads = 128;
-constexpr int kRowMaxDim = 256;
+// D (16x8 fp32) += A (16x16) B (16x8), fragments as the PTX ISA lays them out.
+template <typename C>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
-struct RowSmem {
-  float q[kRowMaxDim];
-  float p[kRowThreads];
-  float red[kRowThreads / 32];
+// Codes to exact fp16 pairs: a code under the exponent of 1024 reads as 1024 + code.
+__device__ __forceinline__ uint32_t codes8(uint32_t biased_pair) {  // u8 in bytes 0 and 2, 0x64 in 1 and 3
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1024 + 128
+  return h2_as_u32(__hsub2(u32_as_h2(biased_pair), off));
+}
+__device__ __forceinline__ uint32_t codes4(uint32_t word, int nibble) {  // nibbles n and n + 4
+  const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1024 + 8
+  return h2_as_u32(__hsub2(u32_as_h2(((word >> (4 * nibble)) & 0x000f000fu) | 0x64006400u), off));
+}
+
+// ------------------------------------------------------------------ geometry
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kM = 16;
+
+template <typename T, int BITS, int DP>
+struct Cfg {
+  static constexpr int kKeys = BITS == 16 ? 16 : 32;  // keys of one warp's tile
+  static constexpr int kUnit = kKeys * kWarps;        // keys of one unit of the axis
+  static constexpr int kRow = DP * BITS / 8;          // bytes of a staged row
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kStages = BITS == 4 ? 4 : 3;
+  static constexpr int kScale = BITS == 16 ? 0 : BITS == 8 ? 4 : 8;  // bytes of a row's scale
+  static constexpr int kVOff = kKeys * kRow;
+  static constexpr int kScOff = 2 * kKeys * kRow;
+  static constexpr int kStage = kScOff + 2 * kKeys * kScale;
+  static constexpr int kWarpBytes = kStages * kStage;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static_assert(kWarpBytes >= kM * DP * 4, "a warp's ring holds its output tile at the end");
+  using C = std::conditional_t<BITS == 16, T, __half>;
+  static constexpr bool kRowFactor = BITS != 16 && std::is_same_v<T, __nv_bfloat16>;
 };
 
-__device__ __forceinline__ float row_reduce(float v, bool is_max, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = is_max ? fmaxf(v, w) : v + w;
+// Where chunk c (16 bytes) of a staged row lies, so that the fragment loads below meet
+// no bank twice: 16-bit rows as ldmatrix wants them; quantised keys are read as whole
+// 16-byte pieces of two neighbouring rows at a time, quantised values as words of rows
+// 2t, t = 0..3, 32 bytes each.
+template <int BITS, int CHUNKS, bool IS_V>
+__device__ __forceinline__ uint32_t chunk_at(int row, int c) {
+  if constexpr (BITS == 16) {
+    return static_cast<uint32_t>(row * CHUNKS + (c ^ (row & 7))) * 16u;
+  } else if constexpr (!IS_V) {
+    return static_cast<uint32_t>(row * CHUNKS + (CHUNKS >= 8 ? c ^ (row & 1) : c)) * 16u;
+  } else {
+    const int l = row * CHUNKS + c;
+    return static_cast<uint32_t>(l ^ (((row >> 1) & 3) << 1)) * 16u;
   }
-  __syncthreads();  // red may still be read by the previous reduction
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = red[0];
-#pragma unroll
-  for (int i = 1; i < kRowThreads / 32; ++i) r = is_max ? fmaxf(r, red[i]) : r + red[i];
-  return r;
 }
 
-// One row by one block of kRowThreads threads, in fp32 throughout: a thread takes whole
-// keys for the scores and then elements of the output. Keys that the row does not see
-// are never read.
-template <typename T, int BITS>
-__device__ void attn_one_row(const AttnArgs& a, int b, const SeqRange& r, int i, int h, RowSmem& sm) {
-  const int D = a.kv.head_dim;
-  const int kvh = h / a.group;
-  const T* q = static_cast<const T*>(a.q) + (r.start + i) * a.q_token_stride + static_cast<int64_t>(h) * D;
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += kRowThreads) sm.q[d] = to_f32(q[d]);
-  __syncthreads();
-  const int pos = r.kv_len - r.q_len + i;
-  const int j1 = min(pos, r.kv_len - 1) + 1;
-  const int j0 = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int mask = (1 << a.kv.page_shift) - 1;
-  float m = -INFINITY, l = 0.f, o[kRowMaxDim / kRowThreads] = {};
-  for (int jb = j0; jb < j1; jb += kRowThreads) {
-    const int j = jb + static_cast<int>(threadIdx.x);
-    float s = -INFINITY;
-    if (j < j1) {
-      const int page = page_of(a, b, j >> a.kv.page_shift);
-      if (page >= 0) {
-        const uint8_t* row = a.kv.k + a.kv.row(page, kvh, j & mask);
-        float step = 1.f, base = 0.f;
-        if constexpr (BITS != 16) {
-          const float* sc = a.kv.k_scale + a.kv.scale_row(page, kvh, j & mask);
-          step = sc[0];
-          if constexpr (BITS == 4) base = sc[1];
-        }
-        float dot = 0.f;
-        for (int c = 0; c < D / 8; ++c) {
-          float x[8];
-          load8<T, BITS>(row, c, step, base, x);
+// What the units of one sequence are: row tiles x KV heads x `units` each, the first at
+// unit t0 of the key axis. Every item has at least one, so that rows that see nothing are
+// written too.
+struct SeqPlan {
+  SeqRange r;
+  int row_tiles, t0, units;
+  __device__ __forceinline__ int64_t total(int kv_heads) const {
+    return static_cast<int64_t>(row_tiles) * kv_heads * units;
+  }
+};
+__device__ __forceinline__ SeqPlan plan_seq(const AttnArgs& a, int b, int unit) {
+  SeqPlan p;
+  p.r = seq_range(a, b);
+  p.row_tiles = (p.r.q_len * a.group + kM - 1) / kM;
+  const int lo = a.window > 0 ? max(0, p.r.kv_len - p.r.q_len - a.window + 1) : 0;
+  p.t0 = lo / unit;
+  p.units = max(1, (p.r.kv_len + unit - 1) / unit - p.t0);
+  return p;
+}
+
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fmaf(sm.q[8 * c + e], x[e], dot);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+// All units of the call (by a whole warp).
+__device__ __forceinline__ int64_t all_units(const AttnArgs& a, int unit, int lane) {
+  int64_t sum = 0;
+  for (int b = lane; b < a.num_seqs; b += 32) sum += plan_seq(a, b, unit).total(a.kv.kv_heads);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+// The sequence that unit u lies in and its first unit; `rows`: the same for row tiles.
+template <typename F>
+__device__ __forceinline__ bool find_seq(const AttnArgs& a, int64_t u, int lane, int& b, int64_t& first, F&& size) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.num_seqs; b0 += 32) {
+    const int64_t n = b0 + lane < a.num_seqs ? size(b0 + lane) : 0;
+    const int64_t incl = base + warp_scan(n, lane);
+    const uint32_t past = __ballot_sync(0xffffffffu, incl > u);
+    if (past != 0) {
+      const int src = __ffs(past) - 1;
+      b = b0 + src;
+      first = __shfl_sync(0xffffffffu, incl - n, src);
+      return true;
+    }
+    base = __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+// Blocks that share the units (each has at least one), unit range of block w of n, and the block that unit u falls to.
+__device__ __forceinline__ int sharing(int64_t units, int blocks) {
+  return static_cast<int>(min(units, static_cast<int64_t>(blocks)));
+}
+__device__ __forceinline__ int64_t first_unit(int64_t units, int w, int n) { return units * w / n; }
+__device__ __forceinline__ int owner(int64_t units, int64_t u, int n) {
+  return static_cast<int>(((u + 1) * n - 1) / units);
+}
+
+// Unnormalised parts of heads that several blocks share: block w's first piece in slot
+// 2 w, a last piece that another block goes on with in 2 w + 1.
+struct Parts {
+  float* o;    // [slots][kM][DP]
+  float2* ml;  // [slots][kM]: reference m, sum l
+};
+
+// ------------------------------------------------------------------ the kernel
+template <typename T, int BITS, int DP>
+__global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const Parts parts) {
+  using K = Cfg<T, BITS, DP>;
+  using C = typename K::C;
+  constexpr int kKeys = K::kKeys, kChunks = K::kChunks, kStages = K::kStages;
+  constexpr int kNt = kKeys / 8;    // score tiles of 8 keys
+  constexpr int kKs = DP / 16;      // k steps of q.k
+  constexpr int kDt = DP / 8;       // output tiles of 8 columns
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_m[kWarps][kM], s_l[kWarps][kM];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, tig = lane & 3;
+  const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * K::kWarpBytes);
+  float* const my_out = reinterpret_cast<float*>(smem + warp * K::kWarpBytes);
+  const int D = a.kv.head_dim;
+  const int row_bytes = D * BITS / 8;
+  const int mask = (1 << a.kv.page_shift) - 1;
+  const float cs = a.scale * kLog2e;
+
+  grid_dep_wait();
+  const int64_t units = all_units(a, K::kUnit, lane);
+  const int blocks = sharing(units, gridDim.x);
+  if (static_cast<int>(blockIdx.x) >= blocks) return;
+  int64_t u = first_unit(units, blockIdx.x, blocks);
+  const int64_t u_end = first_unit(units, blockIdx.x + 1, blocks);
+  bool first_piece = true;
+  int64_t seq_first = 0, seq_end = 0;
+  int b = 0;
+  SeqPlan p{};
+  while (u < u_end) {
+    if (u >= seq_end) {
+      if (!find_seq(a, u, lane, b, seq_first, [&](int s) { return plan_seq(a, s, K::kUnit).total(a.kv.kv_heads); })) break;
+      p = plan_seq(a, b, K::kUnit);
+      seq_end = seq_first + p.total(a.kv.kv_heads);
+    }
+    // the piece: units [tile, tile + cnt) of KV head h, row tile rt
+    const int64_t local = u - seq_first;
+    const int item = static_cast<int>(local / p.units), tile = static_cast<int>(local % p.units);
+    const int rt = item / a.kv.kv_heads, h = item % a.kv.kv_heads;
+    const int cnt = static_cast<int>(min(static_cast<int64_t>(p.units - tile), u_end - u));
+    const int rows = min(kM, p.r.q_len * a.group - rt * kM);
+    const int pos0 = p.r.kv_len - p.r.q_len;  // position of the first new token
+    // this thread's rows, gid and gid + 8: last and first position they see
+    int last[2], from[2];
+    const T* q_row[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = gid + 8 * i;
+      const int tok = (rt * kM + r) / a.group, hh = (rt * kM + r) % a.group;
+      last[i] = r < rows ? pos0 + tok : -1;
+      from[i] = a.window > 0 ? max(0, last[i] - a.window + 1) : 0;
+      q_row[i] = r < rows ? static_cast<const T*>(a.q) + (p.r.start + tok) * a.q_token_stride +
+                                static_cast<int64_t>(h * a.group + hh) * D
+                          : nullptr;
+    }
+    const int tile_min = pos0 + rt * kM / a.group;  // positions of the row tile's first and last row
+    const int tile_max = pos0 + (rt * kM + rows - 1) / a.group;
+
+    // ---------------------------------------------------------- loads
+    auto load = [&](int t) {  // stages this warp's keys of the piece's unit t
+      if (t < cnt) {
+        const uint32_t st = ring + static_cast<uint32_t>(t % kStages) * K::kStage;
+        const int j = (p.t0 + tile + t) * K::kUnit + warp * kKeys + lane;
+        int64_t off = -1, soff = 0;
+        if (lane < kKeys && j < p.r.kv_len) {
+          const int page = page_of(a, b, j >> a.kv.page_shift);
+          if (page >= 0) {
+            off = a.kv.row(page, h, j & mask);
+            if constexpr (BITS != 16) soff = a.kv.scale_row(page, h, j & mask);
+          }
         }
-        s = dot * (a.scale * kLog2e);
+        const bool wide = BITS != 4 || row_bytes % 16 == 0;
+#pragma unroll
+        for (int it = 0; it < kKeys * kChunks / 32; ++it) {
+          const int idx = it * 32 + lane;
+          const int row = idx / kChunks, c = idx % kChunks;
+          const int64_t ro = __shfl_sync(0xffffffffu, off, row);
+          if (c * 16 < row_bytes) {
+            const int64_t src = ro < 0 ? 0 : ro + c * 16;
+            const uint32_t kd = st + chunk_at<BITS, kChunks, false>(row, c);
+            const uint32_t vd = st + K::kVOff + chunk_at<BITS, kChunks, true>(row, c);
+            if (wide) {
+              cp16(kd, a.kv.k + src, ro < 0 ? 0u : 16u);
+              cp16(vd, a.kv.v + src, ro < 0 ? 0u : 16u);
+            } else {  // rows of 8-byte alignment (4 bits, head_dim not a multiple of 32)
+              const bool two = c * 16 + 8 < row_bytes;
+              cp8(kd, a.kv.k + src, ro < 0 ? 0u : 8u);
+              cp8(vd, a.kv.v + src, ro < 0 ? 0u : 8u);
+              if (two) {
+                cp8(kd + 8, a.kv.k + src + (ro < 0 ? 0 : 8), ro < 0 ? 0u : 8u);
+                cp8(vd + 8, a.kv.v + src + (ro < 0 ? 0 : 8), ro < 0 ? 0u : 8u);
+              }
+            }
+          }
+        }
+        if constexpr (BITS != 16) {
+          const uint32_t sd = st + K::kScOff + static_cast<uint32_t>(lane) * K::kScale;
+          constexpr uint32_t kV = kKeys * K::kScale;
+          if constexpr (BITS == 8) {
+            cp4(sd, a.kv.k_scale + soff, off < 0 ? 0u : 4u);
+            cp4(sd + kV, a.kv.v_scale + soff, off < 0 ? 0u : 4u);
+          } else {
+            cp8(sd, a.kv.k_scale + soff, off < 0 ? 0u : 8u);
+            cp8(sd + kV, a.kv.v_scale + soff, off < 0 ? 0u : 8u);
+          }
+        }
+      }
+      cp_commit();
+    };
+    if (BITS == 16 && D < DP) {
+      // columns past head_dim meet zero queries; they must not hold a NaN
+      for (int i = lane; i < kStages * kKeys * (kChunks - row_bytes / 16); i += 32) {
+        const int n = kChunks - row_bytes / 16;
+        const int row = i / n % kKeys, c = row_bytes / 16 + i % n;
+        const uint32_t at = static_cast<uint32_t>(i / n / kKeys) * K::kStage + chunk_at<BITS, kChunks, false>(row, c);
+        *reinterpret_cast<uint4*>(smem + warp * K::kWarpBytes + at) = make_uint4(0, 0, 0, 0);
       }
     }
-    // a NaN score has to reach the sums: fmaxf alone would drop it
-    const float top = fmaxf(m, row_reduce(s, true, sm.red));
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float keep = exp2f(m - ref);
-    const float p = j < j1 ? exp2f(s - ref) : 0.f;
-    sm.p[threadIdx.x] = p;
-    l = l * keep + row_reduce(p, false, sm.red);  // its barriers also publish p
-    m = top;
-    const int cnt = min(kRowThreads, j1 - jb);
 #pragma unroll
-    for (int u = 0; u < kRowMaxDim / kRowThreads; ++u) {
-      const int d = threadIdx.x + u * kRowThreads;
-      if (d >= D) continue;
-      float acc = o[u] * keep;
-      for (int t = 0; t < cnt; ++t) {
-        const int jj = jb + t;
-        const int page = page_of(a, b, jj >> a.kv.page_shift);
-        if (page < 0) continue;
-        const uint8_t* row = a.kv.v + a.kv.row(page, kvh, jj & mask);
-        float x;
-        if constexpr (BITS == 16) {
-          x = to_f32(reinterpret_cast<const T*>(row)[d]);
-        } else {
-          const float* sc = a.kv.v_scale + a.kv.scale_row(page, kvh, jj & mask);
-          if constexpr (BITS == 8) x = static_cast<float>(reinterpret_cast<const int8_t*>(row)[d]) * sc[0];
-          else x = fmaf(static_cast<float>((row[d >> 1] >> (4 * (d & 1))) & 15), sc[0], sc[1]);
-        }
-        acc = fmaf(sm.p[t], x, acc);
+    for (int t = 0; t < kStages - 1; ++t) load(t);
+
+    // ---------------------------------------------------------- queries
+    // Fragment k index <-> element: in order for 16 bits; for codes the order in which a
+    // thread's contiguous quarter row unpacks (a dot product takes any).
+    uint32_t qa[kKs][4];
+    float rf[2] = {1.f, 1.f}, qsum[2] = {0.f, 0.f};
+    if constexpr (K::kRowFactor) {
+      // bf16 queries against fp16 codes: each row scaled by a power of two to at most 2,
+      // which costs only what lies 2^-24 below its largest element
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float most = 0.f;
+        if (q_row[i] != nullptr)
+          for (int d = tig * 8; d < D; d += 32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(q_row[i] + d);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack2<T>(ws[e]);
+              most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = most > 0.f && most < INFINITY ? min(max(ilogbf(most), -126), 126) : 0;
+        rf[i] = exp2f(static_cast<float>(e));
       }
-      o[u] = acc;
+    }
+    auto q2 = [&](int i, int d0, int d1) -> uint32_t {  // elements d0, d1 of row i
+      if (q_row[i] == nullptr) return 0u;
+      if constexpr (!K::kRowFactor) {
+        const uint16_t* x = reinterpret_cast<const uint16_t*>(q_row[i]);
+        const uint32_t lo = d0 < D ? x[d0] : 0u, hi = d1 < D ? x[d1] : 0u;
+        return lo | hi << 16;
+      } else {
+        const float inv = 1.f / rf[i];
+        return pack2<__half>(d0 < D ? to_f32(q_row[i][d0]) * inv : 0.f, d1 < D ? to_f32(q_row[i][d1]) * inv : 0.f);
+      }
+    };
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (BITS == 16) {
+          qa[ks][i] = q2(i, ks * 16 + 2 * tig, ks * 16 + 2 * tig + 1);
+          qa[ks][i + 2] = q2(i, ks * 16 + 2 * tig + 8, ks * 16 + 2 * tig + 9);
+        } else if constexpr (BITS == 8) {
+          const int d = tig * (DP / 4) + 4 * ks;
+          qa[ks][i] = q2(i, d, d + 1);
+          qa[ks][i + 2] = q2(i, d + 2, d + 3);
+        } else {
+          const int d = tig * (DP / 4) + 8 * (ks >> 1) + 2 * (ks & 1);
+          qa[ks][i] = q2(i, d, d + 4);
+          qa[ks][i + 2] = q2(i, d + 1, d + 5);
+          const float2 f = __half22float2(u32_as_h2(qa[ks][i])), g = __half22float2(u32_as_h2(qa[ks][i + 2]));
+          qsum[i] += f.x + f.y + g.x + g.y;
+        }
+      }
+    }
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        qsum[i] += __shfl_xor_sync(0xffffffffu, qsum[i], 1);
+        qsum[i] += __shfl_xor_sync(0xffffffffu, qsum[i], 2);
+      }
+    }
+
+    // ---------------------------------------------------------- the keys
+    float o[kDt][4];
+#pragma unroll
+    for (int i = 0; i < kDt; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, zacc[2] = {0.f, 0.f};
+    for (int t = 0; t < cnt; ++t) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      load(t + kStages - 1);
+      const uint32_t st = ring + static_cast<uint32_t>(t % kStages) * K::kStage;
+      const int j0 = (p.t0 + tile + t) * K::kUnit + warp * kKeys;
+      if (j0 > tile_max) continue;  // nothing here for any row
+      float s[kNt][4];
+#pragma unroll
+      for (int i = 0; i < kNt; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int ks = 0; ks < kKs; ++ks) {
+          uint32_t f[4];
+          ldsm4(st + chunk_at<BITS, kChunks, false>((lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)), f);
+          mma<C>(s[0], qa[ks], f[0], f[1]);
+          mma<C>(s[1], qa[ks], f[2], f[3]);
+        }
+      } else {
+        constexpr int kBytes = DP * BITS / 32;          // of a row, a thread
+        constexpr int kWords = kBytes >= 16 ? 4 : 2;    // a load
+#pragma unroll
+        for (int i = 0; i < kNt; ++i) {
+#pragma unroll
+          for (int n = 0; n < kBytes / (4 * kWords); ++n) {
+            const int byte = tig * kBytes + n * 4 * kWords;
+            uint32_t w[kWords];
+            lds_words<kWords>(st + chunk_at<BITS, kChunks, false>(8 * i + gid, byte >> 4) + (byte & 15), w);
+#pragma unroll
+            for (int e = 0; e < kWords; ++e) {
+              if constexpr (BITS == 8) {
+                const uint32_t x = w[e] ^ 0x80808080u;
+                mma<C>(s[i], qa[n * kWords + e], codes8(__byte_perm(x, 0x64646464u, 0x4140)),
+                       codes8(__byte_perm(x, 0x64646464u, 0x4342)));
+              } else {
+                mma<C>(s[i], qa[2 * (n * kWords + e)], codes4(w[e], 0), codes4(w[e], 1));
+                mma<C>(s[i], qa[2 * (n * kWords + e) + 1], codes4(w[e], 2), codes4(w[e], 3));
+              }
+            }
+          }
+        }
+      }
+      // scores, in powers of two
+      float inv[kNt][2], zr[kNt][2];
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int i = 0; i < kNt; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] *= cs;
+      } else {
+        const float* ksc = reinterpret_cast<const float*>(smem + (st - smem_u32(smem)) + K::kScOff);
+        const float* vsc = ksc + kKeys * K::kScale / 4;
+#pragma unroll
+        for (int i = 0; i < kNt; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = 8 * i + 2 * tig + e;
+            float ks_, kz = 0.f, vs_, vz = 0.f;
+            if constexpr (BITS == 8) {
+              ks_ = ksc[j];
+              vs_ = vsc[j];
+            } else {
+              const float2 kk = reinterpret_cast<const float2*>(ksc)[j], vv = reinterpret_cast<const float2*>(vsc)[j];
+              ks_ = kk.x;
+              kz = fmaf(8.f, kk.x, kk.y);
+              vs_ = vv.x;
+              vz = fmaf(8.f, vv.x, vv.y);
+            }
+            vs_ = vs_ < kMinScale ? kMinScale : vs_;  // a step of zero; a NaN stays
+            const float lv = lg2(vs_);
+            inv[i][e] = 1.f / vs_;
+            zr[i][e] = vz * inv[i][e];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float x = s[i][e + 2 * r] * ks_;
+              if constexpr (BITS == 4) x = fmaf(qsum[r], kz, x);
+              if constexpr (K::kRowFactor) x *= rf[r];
+              s[i][e + 2 * r] = fmaf(x, cs, lv);
+            }
+          }
+      }
+      const bool full = j0 + kKeys - 1 <= tile_min && (a.window <= 0 || j0 > tile_max - a.window);
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < kNt; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = j0 + 8 * i + 2 * tig + (e & 1);
+            if (j > last[e >> 1] || j < from[e >> 1]) s[i][e] = -INFINITY;
+          }
+      }
+      float ref[2], now[2];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int i = 0; i < kNt; ++i) top = fmaxf(top, fmaxf(s[i][2 * r], s[i][2 * r + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        ref[r] = top == -INFINITY ? 0.f : top;
+        now[r] = top;
+        moved |= top != m[r];
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float keep = ex2(m[r] - ref[r]);
+          l[r] *= keep;
+          zacc[r] *= keep;
+#pragma unroll
+          for (int i = 0; i < kDt; ++i) {
+            o[i][2 * r] *= keep;
+            o[i][2 * r + 1] *= keep;
+          }
+          m[r] = now[r];
+        }
+      }
+      uint32_t pa[kKeys / 16][4];
+#pragma unroll
+      for (int i = 0; i < kNt; ++i) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = e >> 1;
+          w[e] = ex2(s[i][e] - ref[r]);
+          if constexpr (BITS == 16) {
+            l[r] += w[e];
+          } else {
+            // what a row does not see may have any step: it stays out of the sums
+            const bool in = full || s[i][e] != -INFINITY;
+            l[r] += in ? w[e] * inv[i][e & 1] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t pair = pack2<C>(w[2 * r], w[2 * r + 1]);
+          pa[i >> 1][(i & 1) * 2 + r] = pair;
+          if constexpr (BITS == 4) {
+            // the rounded weights, so that their rounding scales with the value and not
+            // with the code's distance from 8
+            const float2 f = unpack2<C>(pair);
+            zacc[r] += full || s[i][2 * r] != -INFINITY ? f.x * zr[i][0] : 0.f;
+            zacc[r] += full || s[i][2 * r + 1] != -INFINITY ? f.y * zr[i][1] : 0.f;
+          }
+        }
+      }
+      if constexpr (BITS == 16) {
+        bool odd = false;  // a value that is no number, in a tile that not every row sees whole
+        if (!full) {
+          for (int i = lane; i < kKeys * kChunks; i += 32) {
+            if (i % kChunks * 16 >= row_bytes) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + (st - smem_u32(smem)) + K::kVOff +
+                                                            chunk_at<BITS, kChunks, true>(i / kChunks, i % kChunks));
+            const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack2<T>(ws[e]);
+              odd |= !isfinite(f.x) || !isfinite(f.y);
+            }
+          }
+          odd = __any_sync(0xffffffffu, odd);
+        }
+        if (!odd) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+              uint32_t f[4];
+              ldsm4_t(st + K::kVOff + chunk_at<BITS, kChunks, true>(kk * 16 + (lane & 15), 2 * d + (lane >> 4)), f);
+              mma<C>(o[2 * d], pa[kk], f[0], f[1]);
+              mma<C>(o[2 * d + 1], pa[kk], f[2], f[3]);
+            }
+        } else {
+          // zero times such a value is no number: only rows that see a key may touch it
+          for (int j = 0; j < kKeys; ++j) {
+            const int src = gid * 4 + (j % 8) / 2;
+            float w[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t pair = __shfl_sync(0xffffffffu, j < 8 ? pa[0][r] : pa[0][2 + r], src);
+              const float2 f = unpack2<C>(pair);
+              w[r] = j % 2 ? f.y : f.x;
+            }
+            const bool sees[2] = {j0 + j <= last[0] && j0 + j >= from[0], j0 + j <= last[1] && j0 + j >= from[1]};
+#pragma unroll
+            for (int i = 0; i < kDt; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int d = 8 * i + 2 * tig + e;
+                if (d >= D) continue;
+                const float v = to_f32(*reinterpret_cast<const T*>(smem + (st - smem_u32(smem)) + K::kVOff +
+                                                                   chunk_at<BITS, kChunks, true>(j, d >> 3) + (d & 7) * 2));
+                if (sees[0]) o[i][e] = fmaf(w[0], v, o[i][e]);
+                if (sees[1]) o[i][2 + e] = fmaf(w[1], v, o[i][2 + e]);
+              }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+          for (int n = 0; n < K::kRow / 32; ++n) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = kk * 16 + 2 * tig + (e & 1) + (e >> 1) * 8;
+              w[e] = lds32(st + K::kVOff + chunk_at<BITS, kChunks, true>(row, 2 * n + (gid >> 2)) + (gid & 3) * 4);
+            }
+            if constexpr (BITS == 8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t sel = static_cast<uint32_t>(j | (4 + j) << 8);
+                auto pick = [&](uint32_t x, uint32_t y) {
+                  const uint32_t g = __byte_perm(x, y, (sel & 15u) | (sel >> 8) << 8);
+                  return codes8((g & 0x00ff00ffu) | 0x64006400u);
+                };
+                mma<C>(o[4 * n + j], pa[kk], pick(w[0], w[1]), pick(w[2], w[3]));
+              }
+            } else {
+              const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5410), hi0 = __byte_perm(w[0], w[1], 0x7632);
+              const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5410), hi1 = __byte_perm(w[2], w[3], 0x7632);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                mma<C>(o[8 * n + j], pa[kk], codes4(lo0, j), codes4(lo1, j));
+                mma<C>(o[8 * n + 4 + j], pa[kk], codes4(hi0, j), codes4(hi1, j));
+              }
+            }
+          }
+      }
+    }
+    cp_wait<0>();
+
+    // ---------------------------------------------------------- join the warps, write
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if constexpr (BITS == 4) {
+        zacc[r] += __shfl_xor_sync(0xffffffffu, zacc[r], 1);
+        zacc[r] += __shfl_xor_sync(0xffffffffu, zacc[r], 2);
+      }
+      if (tig == 0) {
+        s_m[warp][gid + 8 * r] = m[r];
+        s_l[warp][gid + 8 * r] = l[r];
+      }
+    }
+    __syncthreads();  // also: every warp has read its last stage
+    float top[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = s_m[0][gid + 8 * r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top[r] = fmaxf(top[r], s_m[w][gid + 8 * r]);
+      const float keep = ex2(m[r] - (top[r] == -INFINITY ? 0.f : top[r]));
+#pragma unroll
+      for (int i = 0; i < kDt; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          int d;  // the column this fragment element stands for
+          if constexpr (BITS == 16) d = 8 * i + 2 * tig + e;
+          else if constexpr (BITS == 8) d = 32 * (i / 4) + 4 * (2 * tig + e) + i % 4;
+          else d = 64 * (i / 8) + 8 * (2 * tig + e) + i % 8;
+          my_out[(gid + 8 * r) * DP + d] = (o[i][2 * r + e] + zacc[r]) * keep;
+        }
     }
     __syncthreads();
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // an empty row gives 0, a NaN one NaN
-  T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(r.start + i) * a.q_heads + h) * D;
+    const bool whole = tile == 0 && cnt == p.units;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1);
+    for (int i = threadIdx.x; i < rows * (DP / 2); i += kThreads) {
+      const int row = i / (DP / 2), d = i % (DP / 2) * 2;
+      if (d >= D) continue;
+      float mm = s_m[0][row];
 #pragma unroll
-  for (int u = 0; u < kRowMaxDim / kRowThreads; ++u) {
-    const int d = threadIdx.x + u * kRowThreads;
-    if (d < D) out[d] = from_f32<T>(o[u] * inv);
+      for (int w = 1; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][row]);
+      const float rr = mm == -INFINITY ? 0.f : mm;
+      float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        sum += s_l[w][row] * ex2(s_m[w][row] - rr);
+        const float2 f = *reinterpret_cast<const float2*>(smem + w * K::kWarpBytes + (row * DP + d) * 4);
+        x += f.x;
+        y += f.y;
+      }
+      if (whole) {
+        const int tok = (rt * kM + row) / a.group, hh = (rt * kM + row) % a.group;
+        const int64_t at = static_cast<int64_t>(p.r.start + tok) * a.q_heads + h * a.group + hh;
+        const float n = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at * D + d) = pack2<T>(x * n, y * n);
+        if (d == 0 && a.lse != nullptr) a.lse[at] = sum == 0.f ? -INFINITY : (mm + log2f(sum)) * kLn2;
+      } else {
+        *reinterpret_cast<float2*>(parts.o + (slot * kM + row) * DP + d) = make_float2(x, y);
+        if (d == 0) parts.ml[slot * kM + row] = make_float2(mm, sum);
+      }
+    }
+    __syncthreads();  // the rings are free again
+    u += cnt;
+    first_piece = false;
   }
-  if (a.lse != nullptr && threadIdx.x == 0)
-    a.lse[static_cast<int64_t>(r.start + i) * a.q_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// One block a row: the simplest form.
-template <typename T, int BITS>
-__global__ void __launch_bounds__(kRowThreads) k_attn_rows(const AttnArgs a) {
-  __shared__ RowSmem sm;
+// Adds up the parts of heads that were cut: block (row tile and KV head, row of the
+// tile). 8 groups of threads take every eighth part; the order of the sums is fixed.
+constexpr int kJoinThreads = 256;
+template <typename T, int BITS, int DP>
+__global__ void __launch_bounds__(kJoinThreads) k_attn_join(const AttnArgs a, const Parts parts, int launched) {
+  using K = Cfg<T, BITS, DP>;
+  constexpr int kCols = DP / 4, kGroups = kJoinThreads / kCols;
+  __shared__ float4 s_o[kGroups][kCols];
+  __shared__ float s_l[kGroups], s_m[kJoinThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_dep_wait();
-  const int h = blockIdx.x % a.q_heads;
-  const int t = blockIdx.x / a.q_heads;
-  for (int b = 0; b < a.num_seqs; ++b) {
-    const SeqRange r = seq_range(a, b);
-    if (t >= r.start && t < r.start + r.q_len) {
-      attn_one_row<T, BITS>(a, b, r, t - r.start, h, sm);
-      return;
-    }
+  const int h = blockIdx.x % a.kv.kv_heads, row = blockIdx.y;
+  const int64_t which = blockIdx.x / a.kv.kv_heads;
+  // (sequence, row tile) number `which`, and the first unit of its sequence
+  int b = 0;
+  int64_t tile_first = 0, unit_base = 0;
+  if (!find_seq(a, which, lane, b, tile_first, [&](int s) { return static_cast<int64_t>(plan_seq(a, s, K::kUnit).row_tiles); }))
+    return;
+  for (int s = lane; s < b; s += 32) unit_base += plan_seq(a, s, K::kUnit).total(a.kv.kv_heads);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) unit_base += __shfl_xor_sync(0xffffffffu, unit_base, o);
+  const int64_t units = all_units(a, K::kUnit, lane);
+  const int blocks = sharing(units, launched);
+  const SeqPlan p = plan_seq(a, b, K::kUnit);
+  const int rt = static_cast<int>(which - tile_first);
+  if (row >= min(kM, p.r.q_len * a.group - rt * kM)) return;
+  const int64_t u0 = unit_base + (static_cast<int64_t>(rt) * a.kv.kv_heads + h) * p.units;
+  const int w0 = owner(units, u0, blocks), w1 = owner(units, u0 + p.units - 1, blocks);
+  if (w0 == w1) return;  // one block had it whole
+  auto slot = [&](int w) -> int64_t {
+    return 2 * static_cast<int64_t>(w) + (w == w0 && first_unit(units, w, blocks) < u0 ? 1 : 0);
+  };
+  float top = -INFINITY;
+  for (int w = w0 + static_cast<int>(threadIdx.x); w <= w1; w += kJoinThreads)
+    top = fmaxf(top, parts.ml[slot(w) * kM + row].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_m[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, s_m[i]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int w = w0 + grp; w <= w1; w += kGroups) {
+    const int64_t s = slot(w) * kM + row;
+    const float2 ml = parts.ml[s];
+    const float4 v = *reinterpret_cast<const float4*>(parts.o + s * DP + col * 4);
+    const float f = ex2(ml.x - ref);
+    l = fmaf(ml.y, f, l);
+    acc.x = fmaf(v.x, f, acc.x);
+    acc.y = fmaf(v.y, f, acc.y);
+    acc.z = fmaf(v.z, f, acc.z);
+    acc.w = fmaf(v.w, f, acc.w);
   }
+  s_o[grp][col] = acc;
+  if (col == 0) s_l[grp] = l;
+  __syncthreads();
+  if (grp != 0 || col * 4 >= a.kv.head_dim) return;
+  for (int g = 1; g < kGroups; ++g) {
+    const float4 v = s_o[g][col];
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+    l += s_l[g];
+  }
+  const int tok = (rt * kM + row) / a.group, hh = (rt * kM + row) % a.group;
+  const int64_t at = static_cast<int64_t>(p.r.start + tok) * a.q_heads + h * a.group + hh;
+  const float n = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  uint2 out;
+  out.x = pack2<T>(acc.x * n, acc.y * n);
+  out.y = pack2<T>(acc.z * n, acc.w * n);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.kv.head_dim + col * 4) = out;
+  if (col == 0 && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------------------------ host
+template <typename T, int BITS, int DP>
+struct Few {
+  using K = Cfg<T, BITS, DP>;
+  static std::atomic<size_t> raised[kMaxDevices];
+  static std::atomic<int> resident;
+
+  // Blocks of the axis: all that are resident at once.
+  static int blocks(cudaError_t* err) {
+    *err = raise_smem_limit(k_attn_few<T, BITS, DP>, K::kSmem, raised);
+    int n = resident.load();
+    if (n == 0 && *err == cudaSuccess) {
+      *err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_few<T, BITS, DP>, kThreads, K::kSmem);
+      n = std::max(1, n);
+      if (*err == cudaSuccess) resident.store(n);
+    }
+    return device_sm_count() * std::max(1, n);
+  }
+  static size_t workspace(cudaError_t* err) {
+    const size_t slots = 2 * static_cast<size_t>(blocks(err));
+    return slots * kM * (DP * sizeof(float) + sizeof(float2));
+  }
+  static cudaError_t launch(const AttnArgs& a, void* ws, cudaStream_t s) {
+    cudaError_t e;
+    const int n = blocks(&e);
+    if (e != cudaSuccess) return e;
+    Parts parts;
+    parts.o = static_cast<float*>(ws);
+    parts.ml = reinterpret_cast<float2*>(parts.o + 2 * static_cast<size_t>(n) * kM * DP);
+    e = launch_dep(k_attn_few<T, BITS, DP>, dim3(static_cast<unsigned>(n)), dim3(kThreads), K::kSmem, s, a, parts);
+    if (e != cudaSuccess) return e;
+    // at most this many row tiles: each sequence may end in a partial one
+    const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.group;
+    const int64_t tiles = std::min<int64_t>(rows, rows / kM + a.num_seqs);
+    return launch_dep(k_attn_join<T, BITS, DP>, dim3(static_cast<unsigned>(tiles * a.kv.kv_heads), static_cast<unsigned>(std::min<int64_t>(kM, rows))),
+                      dim3(kJoinThreads), 0, s, a, parts, n);
+  }
+};
+template <typename T, int BITS, int DP>
+std::atomic<size_t> Few<T, BITS, DP>::raised[kMaxDevices];
+template <typename T, int BITS, int DP>
+std::atomic<int> Few<T, BITS, DP>::resident{0};
+
+template <typename F>
+auto with_few(int bits, bool bf16, int head_dim, F&& f) {
+  auto dim = [&](auto t, auto b) {
+    if (head_dim <= 64) return f(Few<decltype(t), decltype(b)::value, 64>());
+    if (head_dim <= 128) return f(Few<decltype(t), decltype(b)::value, 128>());
+    return f(Few<decltype(t), decltype(b)::value, 256>());
+  };
+  auto form = [&](auto t) {
+    if (bits == 16) return dim(t, std::integral_constant<int, 16>());
+    if (bits == 8) return dim(t, std::integral_constant<int, 8>());
+    return dim(t, std::integral_constant<int, 4>());
+  };
+  return bf16 ? form(__nv_bfloat16()) : form(__half());
 }
 
 }  // namespace
 
-size_t attention_workspace(const AttnArgs&, int, int, int) { return 0; }
+size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int, int) {
+  cudaError_t e = cudaSuccess;
+  return with_few(bits, bf16, a.kv.head_dim, [&](auto k) { return decltype(k)::workspace(&e); });
+}
 
-cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int, int, void*, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.num_tokens) * static_cast<unsigned>(a.q_heads)), block(kRowThreads);
-  if (bf16) {
-    if (bits == 16) return launch_dep(k_attn_rows<__nv_bfloat16, 16>, grid, block, 0, s, a);
-    if (bits == 8) return launch_dep(k_attn_rows<__nv_bfloat16, 8>, grid, block, 0, s, a);
-    return launch_dep(k_attn_rows<__nv_bfloat16, 4>, grid, block, 0, s, a);
-  }
-  if (bits == 16) return launch_dep(k_attn_rows<__half, 16>, grid, block, 0, s, a);
-  if (bits == 8) return launch_dep(k_attn_rows<__half, 8>, grid, block, 0, s, a);
-  return launch_dep(k_attn_rows<__half, 4>, grid, block, 0, s, a);
+cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int, int, void* workspace, cudaStream_t s) {
+  return with_few(bits, bf16, a.kv.head_dim, [&](auto k) { return decltype(k)::launch(a, workspace, s); });
 }
 
 }  // namespace gemq

@@ -82,6 +82,9 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 // Everything an attention launch needs.
 struct AttnArgs {
   KvDev kv;
@@ -139,7 +142,7 @@ cudaError_t launch_cache_write(const KvDev& c, int bits, bool bf16, const void* 
                                cudaStream_t s);
 cudaError_t launch_cache_read(const KvDev& c, int bits, bool bf16, const int64_t* slots, int tokens, void* k, void* v,
                               cudaStream_t s);
-size_t attention_workspace(const AttnArgs& a, int bits, int max_q_len, int max_kv_len);
+size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len);
 cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
                              cudaStream_t s);
 size_t verify_workspace(int B, int n, int V);

@@ -180,6 +180,7 @@ size_t gemq_paged_attention_workspace_size(const gemq_kv_cache_t* cache, int64_t
     if (const int rc = check_attention(cache, num_tokens, q_heads, num_seqs, max_pages, max_q_len, max_kv_len)) return rc;
     if (num_tokens == 0 || num_seqs == 0) return GEMQ_OK;
     bytes = attention_workspace(attn_sizes(cache, num_tokens, q_heads, num_seqs, max_pages), cache->bits,
+                                cache->dtype == GEMQ_BF16,
                                 bound_q(max_q_len, num_tokens), bound_kv(cache, max_kv_len, max_pages));
     return GEMQ_OK;
   });
@@ -205,7 +206,7 @@ int gemq_paged_attention(const gemq_kv_cache_t* cache, const void* q, int64_t q_
       return fail(GEMQ_ERR_UNSUPPORTED, "q and out must start on a 16-byte boundary, q's token stride be a multiple of 8");
     AttnArgs a = attn_sizes(cache, num_tokens, q_heads, num_seqs, max_pages);
     const int mq = bound_q(max_q_len, num_tokens), mk = bound_kv(cache, max_kv_len, max_pages);
-    const size_t need = attention_workspace(a, cache->bits, mq, mk);
+    const size_t need = attention_workspace(a, cache->bits, cache->dtype == GEMQ_BF16, mq, mk);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
       return fail(GEMQ_ERR_WORKSPACE, "workspace too small or unaligned");
     a.q = q;
