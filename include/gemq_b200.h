@@ -429,8 +429,8 @@ int gemq_paged_attention(const gemq_kv_cache_t* cache /* host */, const void* q,
  * tokens int64 [B, n + 1]: the taken drafts, the drawn token, then -1; num_accepted int32
  * [B]; logprobs fp32 [B, n + 1]: log softmax(logits / T) of each token (T = 1 where the
  * temperature is 0), 0 beside a -1. A row with a NaN, a +inf or nothing finite, or a
- * temperature below zero or NaN, has no distribution: its draft is not taken and the
- * token drawn there is -1. A draft outside the vocabulary is not taken.
+ * temperature that is negative or not finite, has no distribution: its draft is not
+ * taken and the token drawn there is -1. A draft outside the vocabulary is not taken.
  * 1 <= num_drafts <= 63, num_seqs <= 65535, vocab < 2^30. */
 typedef struct gemq_verify {
   const void* logits;         /* [num_seqs][num_drafts + 1][vocab] */

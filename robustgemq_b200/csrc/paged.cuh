@@ -85,6 +85,12 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Everything an attention launch needs.
 struct AttnArgs {
   KvDev kv;

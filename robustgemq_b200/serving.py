@@ -33,9 +33,22 @@ def _need(ok: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
-def _on(device: torch.device):
-    """Context in which ``device`` is current (nothing to do when it is)."""
-    return torch.cuda.device(device)
+# These calls are short: on small inputs the host's part of a call is its time. So the
+# argument checks build no message unless they fail, and the stream and the current
+# device are asked of torch directly.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else lambda: -1
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _run(index: int, fn, *args) -> None:
+    """``fn(*args, stream)`` with device ``index`` current, on its current stream."""
+    if _current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)
 
 
 class PagedKVCache:
@@ -80,56 +93,65 @@ class PagedKVCache:
         return self
 
     def _bind(self, k, v, k_scale, v_scale, dtype):
-        _need(k.is_cuda, "k must be a CUDA tensor (no CPU path)")
-        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
-              "k and v must be alike: [num_pages, num_kv_heads, page_size, head_dim]")
-        bits = 8 if k.dtype == torch.int8 else 4 if k.dtype == torch.uint8 else 16
-        _need(dtype in (torch.float16, torch.bfloat16), "dtype must be float16 or bfloat16")
-        _need(bits != 16 or k.dtype == dtype, "a 16-bit cache holds its dtype")
-        strides = k.stride()
-        _need(strides[3] == 1, "rows must be contiguous")
-        pages, heads, page, width = k.shape
+        shape, strides, kind, dev = k.shape, k.stride(), k.dtype, k.device
+        if not k.is_cuda:
+            raise ValueError("k must be a CUDA tensor (no CPU path)")
+        if len(shape) != 4 or v.shape != shape or v.stride() != strides or v.dtype != kind or v.device != dev:
+            raise ValueError("k and v must be alike: [num_pages, num_kv_heads, page_size, head_dim] on one device")
+        code = _CODES.get(dtype)
+        if code is None or code == _lib.FP32:
+            raise ValueError("dtype must be float16 or bfloat16")
+        if strides[3] != 1:
+            raise ValueError("rows must be contiguous")
         c = KvCacheT()
-        c.k, c.v = k.data_ptr(), v.data_ptr()
-        size = k.element_size()
-        c.strides = (strides[0] * size, strides[1] * size, strides[2] * size)
-        devices = [v.device]
-        if bits == 16:
-            _need(k_scale is None and v_scale is None, "a 16-bit cache has no scales")
-        else:
-            want = k.shape[:3] if bits == 8 else k.shape[:3] + (2,)
-            _need(k_scale is not None and v_scale is not None and k_scale.dtype == v_scale.dtype == torch.float32
-                  and k_scale.shape == v_scale.shape == want and k_scale.stride() == v_scale.stride(),
-                  f"k_scale and v_scale must be float32 {tuple(want)} with the same strides")
+        pages, heads, page, dim = shape
+        if kind is torch.int8 or kind is torch.uint8:
+            bits, size = (8, 1) if kind is torch.int8 else (4, 1)
+            want = shape[:3] if bits == 8 else shape[:3] + (2,)
+            if k_scale is None or v_scale is None:
+                raise ValueError("a quantised cache needs k_scale and v_scale")
             ss = k_scale.stride()
-            _need(bits == 8 or ss[3] == 1, "a row's step and base must be neighbours")
+            if not (k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and k_scale.shape == want and
+                    v_scale.shape == want and v_scale.stride() == ss and k_scale.device == dev and
+                    v_scale.device == dev):
+                raise ValueError(f"k_scale and v_scale must be float32 {tuple(want)} with the same strides, beside k")
+            if bits == 4:
+                if ss[3] != 1:
+                    raise ValueError("a row's step and base must be neighbours")
+                dim *= 2
             c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
             c.scale_strides = ss[:3]
-            devices += [k_scale.device, v_scale.device]
-        _need(all(d == k.device for d in devices), "all tensors of a cache must be on one device")
-        c.num_pages, c.kv_heads, c.page_size = pages, heads, page
-        c.head_dim = width * 2 if bits == 4 else width
-        c.bits, c.dtype = bits, _CODES[dtype]
+        else:
+            bits, size = 16, 2
+            if kind is not dtype:
+                raise ValueError("a 16-bit cache holds its dtype")
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("a 16-bit cache has no scales")
+        c.k, c.v = k.data_ptr(), v.data_ptr()
+        c.strides = (strides[0] * size, strides[1] * size, strides[2] * size)
+        c.num_pages, c.kv_heads, c.page_size, c.head_dim, c.bits, c.dtype = pages, heads, page, dim, bits, code
         self.k, self.v, self.k_scale, self.v_scale, self.dtype = k, v, k_scale, v_scale, dtype
         self.bits, self.num_pages, self.num_kv_heads, self.page_size = bits, pages, heads, page
-        self.head_dim, self.device = c.head_dim, k.device
+        self.head_dim, self.device = dim, dev
+        self._index = dev.index
         self._c = c
         self._ref = ctypes.byref(c)
 
     def _check_rows(self, t: Tensor, name: str, tokens: int) -> Tensor:
-        _need(t.dtype == self.dtype and t.device == self.device, f"{name} must be {self.dtype} on the cache's device")
-        _need(t.dim() == 3 and t.shape == (tokens, self.num_kv_heads, self.head_dim),
-              f"{name} must be [tokens, num_kv_heads, head_dim]")
+        if t.dtype is not self.dtype or t.device != self.device:
+            raise ValueError(f"{name} must be {self.dtype} on the cache's device")
+        if t.shape != (tokens, self.num_kv_heads, self.head_dim):
+            raise ValueError(f"{name} must be [tokens, num_kv_heads, head_dim]")
         st = t.stride()
         # rows of another layout (a transposed view) are copied once
-        if st[2] != 1 or st[0] % 8 or st[1] % 8 or st[0] < 0 or t.data_ptr() % 16:
+        if st[2] != 1 or st[0] % 8 or st[1] % 8 or t.data_ptr() % 16:
             return t.contiguous()
         return t
 
     def _check_slots(self, slots: Tensor) -> Tensor:
-        _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.device == self.device,
-              "slots must be int64 [tokens] on the cache's device")
-        return slots.contiguous()
+        if slots.dtype is not torch.int64 or slots.dim() != 1 or slots.device != self.device:
+            raise ValueError("slots must be int64 [tokens] on the cache's device")
+        return slots if slots.is_contiguous() else slots.contiguous()
 
     def write(self, k: Tensor, v: Tensor, slots: Tensor) -> None:
         """Quantises token ``t``'s rows ``k[t]``, ``v[t]`` (``[tokens, num_kv_heads,
@@ -139,21 +161,18 @@ class PagedKVCache:
         tokens = slots.shape[0]
         k, v = self._check_rows(k, "k", tokens), self._check_rows(v, "v", tokens)
         ks, vs = k.stride(), v.stride()
-        with _on(self.device):
-            check(_lib.load().gemq_kv_cache_write(self._ref, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
-                                                  slots.data_ptr(), tokens, _lib.stream_ptr(self.device)))
+        _run(self._index, _lib.load().gemq_kv_cache_write, self._ref, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0],
+             vs[1], slots.data_ptr(), tokens)
 
     def read(self, slots: Tensor) -> Tuple[Tensor, Tensor]:
         """The stored keys and values of ``slots``, ``[tokens, num_kv_heads, head_dim]`` in
         the cache's ``dtype``; zeros for a negative slot."""
         slots = self._check_slots(slots)
-        tokens = slots.shape[0]
-        shape = (2, tokens, self.num_kv_heads, self.head_dim)
-        out = torch.empty(shape, dtype=self.dtype, device=self.device)
-        k, v = out[0], out[1]
-        with _on(self.device):
-            check(_lib.load().gemq_kv_cache_read(self._ref, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
-                                                 _lib.stream_ptr(self.device)))
+        shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=self.dtype, device=self.device)
+        v = torch.empty(shape, dtype=self.dtype, device=self.device)
+        _run(self._index, _lib.load().gemq_kv_cache_read, self._ref, slots.data_ptr(), shape[0], k.data_ptr(),
+             v.data_ptr())
         return k, v
 
 
@@ -179,36 +198,41 @@ def paged_attention(q: Tensor, cache: PagedKVCache, page_table: Tensor, kv_lens:
     ``[tokens, q_heads]``.
     """
     dev = cache.device
-    _need(q.dim() == 3 and q.dtype == cache.dtype and q.device == dev and q.shape[2] == cache.head_dim,
-          "q must be [tokens, q_heads, head_dim] of the cache's dtype and device")
-    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == dev,
-          "page_table must be int32 [seqs, pages] on the cache's device")
+    tokens, heads, dim = shape = q.shape if q.dim() == 3 else (0, 0, -1)
+    if q.dtype is not cache.dtype or q.device != dev or dim != cache.head_dim:
+        raise ValueError("q must be [tokens, q_heads, head_dim] of the cache's dtype and device")
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.device != dev:
+        raise ValueError("page_table must be int32 [seqs, pages] on the cache's device")
     seqs, pages = page_table.shape
-    _need(kv_lens.dtype == torch.int32 and kv_lens.shape == (seqs,) and kv_lens.device == dev,
-          "kv_lens must be int32 [seqs] on the cache's device")
+    if kv_lens.dtype is not torch.int32 or kv_lens.shape != (seqs,) or kv_lens.device != dev:
+        raise ValueError("kv_lens must be int32 [seqs] on the cache's device")
+    starts = None
     if q_starts is not None:
-        _need(q_starts.dtype == torch.int32 and q_starts.shape == (seqs + 1,) and q_starts.device == dev,
-              "q_starts must be int32 [seqs + 1] on the cache's device")
+        if q_starts.dtype is not torch.int32 or q_starts.shape != (seqs + 1,) or q_starts.device != dev:
+            raise ValueError("q_starts must be int32 [seqs + 1] on the cache's device")
         q_starts = q_starts.contiguous()
+        starts = q_starts.data_ptr()
     kv_lens = kv_lens.contiguous()
-    if page_table.stride(1) != 1 or page_table.stride(0) < 0:
+    ts = page_table.stride()
+    if ts[1] != 1:
         page_table = page_table.contiguous()
-    tokens, heads, dim = q.shape
+        ts = page_table.stride()
     st = q.stride()
     if st[2] != 1 or (st[1] != dim and heads != 1) or st[0] % 8 or q.data_ptr() % 16:
         q = q.contiguous()
         st = q.stride()
     lib = _lib.load()
-    out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
+    out = torch.empty(shape, dtype=q.dtype, device=dev)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
-    with _on(dev):
+    if cache._index != _current_device():
+        with torch.cuda.device(cache._index):
+            need = lib.gemq_paged_attention_workspace_size(cache._ref, tokens, heads, seqs, pages, max_q_len, max_kv_len)
+    else:
         need = lib.gemq_paged_attention_workspace_size(cache._ref, tokens, heads, seqs, pages, max_q_len, max_kv_len)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        check(lib.gemq_paged_attention(
-            cache._ref, q.data_ptr(), st[0], tokens, heads, page_table.data_ptr(), page_table.stride(0), pages,
-            kv_lens.data_ptr(), None if q_starts is None else q_starts.data_ptr(), seqs, max_q_len, max_kv_len,
-            dim ** -0.5 if scale is None else scale, window, out.data_ptr(), None if lse is None else lse.data_ptr(),
-            None if ws is None else ws.data_ptr(), need, _lib.stream_ptr(dev)))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _run(cache._index, lib.gemq_paged_attention, cache._ref, q.data_ptr(), st[0], tokens, heads, page_table.data_ptr(),
+         ts[0], pages, kv_lens.data_ptr(), starts, seqs, max_q_len, max_kv_len, dim ** -0.5 if scale is None else scale,
+         window, out.data_ptr(), None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
@@ -241,54 +265,54 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
     ``weight / noise`` (lowest index on ties). A row of logits with a NaN, a +inf or
     nothing finite takes no draft and gives the token -1.
     """
-    _need(target_logits.is_cuda and target_logits.dim() == 3 and target_logits.dtype in _CODES,
-          "target_logits must be a CUDA tensor [seqs, drafts + 1, vocab] of float16, bfloat16 or float32")
+    if not target_logits.is_cuda or target_logits.dim() != 3 or target_logits.dtype not in _CODES:
+        raise ValueError("target_logits must be a CUDA tensor [seqs, drafts + 1, vocab] of float16, bfloat16 or float32")
     dev = target_logits.device
     B, rows, V = target_logits.shape
     n = rows - 1
-    _need(draft_tokens.dtype == torch.int64 and draft_tokens.shape == (B, n) and draft_tokens.device == dev,
-          "draft_tokens must be int64 [seqs, drafts] beside target_logits")
-    _need(uniforms.dtype == torch.float32 and uniforms.shape == (B, n) and uniforms.device == dev,
-          "uniforms must be float32 [seqs, drafts] beside target_logits")
-    _need(noise.dtype == torch.float32 and noise.shape == (B, V) and noise.device == dev,
-          "noise must be float32 [seqs, vocab] beside target_logits")
+    if draft_tokens.dtype is not torch.int64 or draft_tokens.shape != (B, n) or draft_tokens.device != dev:
+        raise ValueError("draft_tokens must be int64 [seqs, drafts] beside target_logits")
+    if uniforms.dtype is not torch.float32 or uniforms.shape != (B, n) or uniforms.device != dev:
+        raise ValueError("uniforms must be float32 [seqs, drafts] beside target_logits")
+    if noise.dtype is not torch.float32 or noise.shape != (B, V) or noise.device != dev:
+        raise ValueError("noise must be float32 [seqs, vocab] beside target_logits")
+    # (names bound to copies live until the call has been issued)
     v = VerifyT()
-    keep = []  # tensors whose copies the call reads
-
-    def dense(t):
-        t = t.contiguous()
-        keep.append(t)
-        return t.data_ptr()
-
-    def strided(t):
-        st = t.stride()
-        if (st[2] != 1 and t.shape[2] != 1) or min(st) < 0:
-            t = t.contiguous()
-            keep.append(t)
-            st = t.stride()
-        return t.data_ptr(), st[0], st[1], _CODES[t.dtype]
-
-    v.logits, v.logits_seq_stride, v.logits_row_stride, v.logits_dtype = strided(target_logits)
+    st = target_logits.stride()
+    if st[2] != 1:
+        target_logits = target_logits.contiguous()
+        st = target_logits.stride()
+    v.logits, v.logits_seq_stride, v.logits_row_stride = target_logits.data_ptr(), st[0], st[1]
+    v.logits_dtype = _CODES[target_logits.dtype]
     if draft_probs is not None:
-        _need(draft_probs.dtype in _CODES and draft_probs.shape == (B, n, V) and draft_probs.device == dev,
-              "draft_probs must be [seqs, drafts, vocab] of float16, bfloat16 or float32 beside target_logits")
-        v.draft_probs, v.probs_seq_stride, v.probs_row_stride, v.probs_dtype = strided(draft_probs)
+        if draft_probs.dtype not in _CODES or draft_probs.shape != (B, n, V) or draft_probs.device != dev:
+            raise ValueError("draft_probs must be [seqs, drafts, vocab] of float16, bfloat16 or float32 beside "
+                             "target_logits")
+        st = draft_probs.stride()
+        if st[2] != 1:
+            draft_probs = draft_probs.contiguous()
+            st = draft_probs.stride()
+        v.draft_probs, v.probs_seq_stride, v.probs_row_stride = draft_probs.data_ptr(), st[0], st[1]
+        v.probs_dtype = _CODES[draft_probs.dtype]
     if draft_lens is not None:
-        _need(draft_lens.dtype == torch.int32 and draft_lens.shape == (B,) and draft_lens.device == dev,
-              "draft_lens must be int32 [seqs] beside target_logits")
-        v.draft_lens = dense(draft_lens)
+        if draft_lens.dtype is not torch.int32 or draft_lens.shape != (B,) or draft_lens.device != dev:
+            raise ValueError("draft_lens must be int32 [seqs] beside target_logits")
+        draft_lens = draft_lens.contiguous()
+        v.draft_lens = draft_lens.data_ptr()
     if temperature is not None:
-        _need(temperature.dtype == torch.float32 and temperature.shape == (B,) and temperature.device == dev,
-              "temperature must be float32 [seqs] beside target_logits")
-        v.temperature = dense(temperature)
-    v.draft_tokens, v.uniforms, v.noise = dense(draft_tokens), dense(uniforms), dense(noise)
-    tokens = torch.empty((B, n + 1), dtype=torch.int64, device=dev)
+        if temperature.dtype is not torch.float32 or temperature.shape != (B,) or temperature.device != dev:
+            raise ValueError("temperature must be float32 [seqs] beside target_logits")
+        temperature = temperature.contiguous()
+        v.temperature = temperature.data_ptr()
+    draft_tokens, uniforms, noise = draft_tokens.contiguous(), uniforms.contiguous(), noise.contiguous()
+    v.draft_tokens, v.uniforms, v.noise = draft_tokens.data_ptr(), uniforms.data_ptr(), noise.data_ptr()
+    tokens = torch.empty((B, rows), dtype=torch.int64, device=dev)
     accepted = torch.empty((B,), dtype=torch.int32, device=dev)
-    logprobs = torch.empty((B, n + 1), dtype=torch.float32, device=dev)
+    logprobs = torch.empty((B, rows), dtype=torch.float32, device=dev)
     v.tokens, v.num_accepted, v.logprobs = tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr()
     lib = _lib.load()
-    with _on(dev):
-        need = lib.gemq_verify_draft_workspace_size(B, n, V)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
-        check(lib.gemq_verify_draft(ctypes.byref(v), B, n, V, ws.data_ptr(), need, _lib.stream_ptr(dev)))
+    index = dev.index
+    need = lib.gemq_verify_draft_workspace_size(B, n, V)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _run(index, lib.gemq_verify_draft, ctypes.byref(v), B, n, V, ws.data_ptr(), need)
     return Verified(tokens, accepted, logprobs)
