@@ -362,8 +362,8 @@ int gemq_decode_attention(const uint16_t* q, const uint16_t* k_cache, const uint
  *            value = code * step + base.
  * Limits: head_dim a multiple of 16, at most 256; page_size a power of two, at most
  * 65536; num_pages * page_size below 2^31; k, v and the code strides multiples of 16
- * bytes (8 for bits 4 with head_dim % 32 != 0); scales 4-byte (bits 8) or 8-byte (bits 4)
- * aligned.
+ * bytes (8 for bits 4 with head_dim % 32 != 0) and below 2^34 bytes; scales 4-byte (bits
+ * 8) or 8-byte (bits 4) aligned, their strides below 2^31. Steps are not negative.
  */
 typedef struct gemq_kv_cache {
   void* k;

@@ -7,13 +7,17 @@
 // A row that sees nothing gives o = 0 and lse = -inf. What a row does not see does not
 // reach it whatever it holds.
 //
-// Quantised rows, k_j = s_j c_j (8 bits) or s_j (c_j - 8) + z_j (4 bits, z_j the value of
-// code 8), and the same for v with step t_j and value y_j of code 8, go to the tensor
-// cores as their codes, which are exact in fp16:
+// Quantised rows k_j = s_j c_j + z_j and v_j = t_j d_j + y_j go to the tensor cores as
+// their codes, which are exact in fp16:
 //   q.k_j = s_j (q.c_j) + z_j sum(q)
-//   o = sum_j w'_j (c_j + y_j / t_j) / sum_j w'_j / t_j,  w'_j = 2^(x_j + log2 t_j - m)
+//   o = sum_j w'_j (d_j + y_j / t_j) / sum_j w'_j / t_j,  w'_j = 2^(x_j + log2 t_j - m)
 // so the value's step acts as a shift of the score, w' stays in [0, 1], and the only
-// rounding below 32 bits is that of w' to 16 bits, as without quantisation.
+// rounding below 32 bits is that of w' to 16 bits, as without quantisation. An unsigned
+// code in the low bits of a half with zero exponent is the subnormal code 2^-24, exactly,
+// and costs one mask; keys take that form at both widths (8 bits as c + 128, with z_j =
+// -128 s_j). Values become signed halves (4 bits: c - 8, y_j the value of code 8): a bias
+// would stand in the sums as a multiple of sum w' that cancels, at 8 bits against long
+// contexts' small averages, at 4 bits where a value is near zero.
 //
 // This file: few rows a KV head (decode steps, drafted tokens), where the cache's bytes
 // are the time. mma.sync with the 16 rows of one KV head (tokens x query heads that share
@@ -62,24 +66,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
                : "r"(a)
                : "memory");
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-template <int N>
-__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
-  if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
-  } else {
-    static_assert(N == 4, "two or four words");
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(a)
-                 : "memory");
-  }
-}
-
 // D (16x8 fp32) += A (16x16) B (16x8), fragments as the PTX ISA lays them out.
 template <typename C>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -97,14 +83,18 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes to exact fp16 pairs: a code under the exponent of 1024 reads as 1024 + code.
-__device__ __forceinline__ uint32_t codes8(uint32_t biased_pair) {  // u8 in bytes 0 and 2, 0x64 in 1 and 3
-  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1024 + 128
-  return h2_as_u32(__hsub2(u32_as_h2(biased_pair), off));
+// Codes of a pair of words with bits 4 S..4 S + 3 in each half (S = 0, 1), minus 8.
+template <int S>
+__device__ __forceinline__ uint32_t signed4(uint32_t w) {
+  // under the exponents of 2^10 and 2^6 the code reads as 1024 + c, 64 + c
+  constexpr uint32_t kMask = S ? 0x00f000f0u : 0x000f000fu, kExp = S ? 0x54005400u : 0x64006400u;
+  constexpr uint32_t kOff = S ? 0x54805480u : 0x64086408u;  // 64 + 8, 1024 + 8
+  return h2_as_u32(__hsub2(u32_as_h2((w & kMask) | kExp), u32_as_h2(kOff)));
 }
-__device__ __forceinline__ uint32_t codes4(uint32_t word, int nibble) {  // nibbles n and n + 4
-  const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1024 + 8
-  return h2_as_u32(__hsub2(u32_as_h2(((word >> (4 * nibble)) & 0x000f000fu) | 0x64006400u), off));
+// Bytes c + 128 in places 0 and 2 of a word, 0x64 in 1 and 3 (1024 + c + 128), to c.
+__device__ __forceinline__ uint32_t signed8(uint32_t pair) {
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  return h2_as_u32(__hsub2(u32_as_h2(pair), off));
 }
 
 // ------------------------------------------------------------------ geometry
@@ -118,12 +108,15 @@ struct Cfg {
   static constexpr int kUnit = kKeys * kWarps;        // keys of one unit of the axis
   static constexpr int kRow = DP * BITS / 8;          // bytes of a staged row
   static constexpr int kChunks = kRow / 16;
-  static constexpr int kStages = BITS == 4 ? 4 : 3;
+  static constexpr int kBlocks = DP == 256 ? 1 : 3;   // resident on an SM
+  static constexpr int kStages = DP * BITS >= 4096 ? 3 : DP * BITS >= 1024 ? 2 : 3;
   static constexpr int kScale = BITS == 16 ? 0 : BITS == 8 ? 4 : 8;  // bytes of a row's scale
   static constexpr int kVOff = kKeys * kRow;
   static constexpr int kScOff = 2 * kKeys * kRow;
   static constexpr int kStage = kScOff + 2 * kKeys * kScale;
-  static constexpr int kWarpBytes = kStages * kStage;
+  // a tile's scales as the scores take them: [keys] each of a, log2 step, 1 / step, z, y / step
+  static constexpr int kPrep = BITS == 16 ? 0 : 5 * kKeys * 4;
+  static constexpr int kWarpBytes = kStages * kStage + kPrep;
   static constexpr int kSmem = kWarps * kWarpBytes;
   static_assert(kWarpBytes >= kM * DP * 4, "a warp's ring holds its output tile at the end");
   using C = std::conditional_t<BITS == 16, T, __half>;
@@ -219,7 +212,7 @@ struct Parts {
 
 // ------------------------------------------------------------------ the kernel
 template <typename T, int BITS, int DP>
-__global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const Parts parts) {
+__global__ void __launch_bounds__(kThreads, Cfg<T, BITS, DP>::kBlocks) k_attn_few(const AttnArgs a, const Parts parts) {
   using K = Cfg<T, BITS, DP>;
   using C = typename K::C;
   constexpr int kKeys = K::kKeys, kChunks = K::kChunks, kStages = K::kStages;
@@ -232,12 +225,15 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
   const int gid = lane >> 2, tig = lane & 3;
   const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * K::kWarpBytes);
   float* const my_out = reinterpret_cast<float*>(smem + warp * K::kWarpBytes);
+  float* const prep = reinterpret_cast<float*>(smem + warp * K::kWarpBytes + kStages * K::kStage);
   const int D = a.kv.head_dim;
   const int row_bytes = D * BITS / 8;
   const int mask = (1 << a.kv.page_shift) - 1;
   const float cs = a.scale * kLog2e;
 
   grid_dep_wait();
+  // every block of this grid is resident, so the join's may be placed beside them now
+  grid_dep_launch();
   const int64_t units = all_units(a, K::kUnit, lane);
   const int blocks = sharing(units, gridDim.x);
   if (static_cast<int>(blockIdx.x) >= blocks) return;
@@ -277,38 +273,89 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
     const int tile_max = pos0 + (rt * kM + rows - 1) / a.group;
 
     // ---------------------------------------------------------- loads
-    auto load = [&](int t) {  // stages this warp's keys of the piece's unit t
+    // Stages this warp's keys of the piece's unit t. Where a page holds whole tiles, one
+    // page id serves a tile (and the next one's is asked for a tile ahead).
+    const bool one_page = (1 << a.kv.page_shift) >= kKeys;
+    const int tile_key = (p.t0 + tile) * K::kUnit + warp * kKeys;
+    const int32_t* const table = a.page_table + b * a.page_table_stride;
+    auto page_at = [&](int t) {
+      const int j = tile_key + t * K::kUnit;
+      return t < cnt && j < p.r.kv_len ? __ldg(table + (j >> a.kv.page_shift)) : -1;
+    };
+    int next_page = one_page ? page_at(0) : -1;
+    constexpr int kRowsIt = 32 / kChunks;  // rows of one step of a warp's copies
+    auto load = [&](int t) {
       if (t < cnt) {
         const uint32_t st = ring + static_cast<uint32_t>(t % kStages) * K::kStage;
-        const int j = (p.t0 + tile + t) * K::kUnit + warp * kKeys + lane;
-        int64_t off = -1, soff = 0;
-        if (lane < kKeys && j < p.r.kv_len) {
-          const int page = page_of(a, b, j >> a.kv.page_shift);
-          if (page >= 0) {
-            off = a.kv.row(page, h, j & mask);
-            if constexpr (BITS != 16) soff = a.kv.scale_row(page, h, j & mask);
-          }
-        }
+        const int j0 = tile_key + t * K::kUnit;
         const bool wide = BITS != 4 || row_bytes % 16 == 0;
-#pragma unroll
-        for (int it = 0; it < kKeys * kChunks / 32; ++it) {
-          const int idx = it * 32 + lane;
-          const int row = idx / kChunks, c = idx % kChunks;
-          const int64_t ro = __shfl_sync(0xffffffffu, off, row);
+        int64_t soff = 0;
+        int live;
+        if (one_page) {
+          const int page = next_page;
+          next_page = page_at(t + 1);
+          live = p.r.kv_len - j0;
+          if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.kv.num_pages)) {
+            if (live > 0) set_device_error(kDevBadCachePos);
+            live = 0;
+          }
+          const int off = j0 & mask;
+          const int row0 = lane / kChunks, c = lane % kChunks;
+          int64_t src = live > 0 ? a.kv.row(page, h, off + row0) + c * 16 : 0;
+          const int64_t step = live > 0 ? static_cast<int64_t>(a.kv.token_stride) * (8 * kRowsIt) : 0;
+          if constexpr (BITS != 16) soff = live > 0 ? a.kv.scale_row(page, h, off + lane) : 0;
           if (c * 16 < row_bytes) {
-            const int64_t src = ro < 0 ? 0 : ro + c * 16;
-            const uint32_t kd = st + chunk_at<BITS, kChunks, false>(row, c);
-            const uint32_t vd = st + K::kVOff + chunk_at<BITS, kChunks, true>(row, c);
-            if (wide) {
-              cp16(kd, a.kv.k + src, ro < 0 ? 0u : 16u);
-              cp16(vd, a.kv.v + src, ro < 0 ? 0u : 16u);
-            } else {  // rows of 8-byte alignment (4 bits, head_dim not a multiple of 32)
-              const bool two = c * 16 + 8 < row_bytes;
-              cp8(kd, a.kv.k + src, ro < 0 ? 0u : 8u);
-              cp8(vd, a.kv.v + src, ro < 0 ? 0u : 8u);
-              if (two) {
-                cp8(kd + 8, a.kv.k + src + (ro < 0 ? 0 : 8), ro < 0 ? 0u : 8u);
-                cp8(vd + 8, a.kv.v + src + (ro < 0 ? 0 : 8), ro < 0 ? 0u : 8u);
+#pragma unroll
+            for (int it = 0; it < kKeys / kRowsIt; ++it) {
+              const int row = it * kRowsIt + row0;
+              const uint32_t kd = st + chunk_at<BITS, kChunks, false>(row, c);
+              const uint32_t vd = st + K::kVOff + chunk_at<BITS, kChunks, true>(row, c);
+              if (wide) {
+                const uint32_t n = row < live ? 16u : 0u;
+                cp16(kd, a.kv.k + src, n);
+                cp16(vd, a.kv.v + src, n);
+              } else {  // rows of 8-byte alignment (4 bits, head_dim not a multiple of 32)
+                const uint32_t n = row < live ? 8u : 0u;
+                cp8(kd, a.kv.k + src, n);
+                cp8(vd, a.kv.v + src, n);
+                if (c * 16 + 8 < row_bytes) {
+                  cp8(kd + 8, a.kv.k + src + 8, n);
+                  cp8(vd + 8, a.kv.v + src + 8, n);
+                }
+              }
+              src += step;
+            }
+          }
+          live -= lane;
+        } else {
+          const int j = j0 + lane;
+          int64_t off = -1;
+          if (lane < kKeys && j < p.r.kv_len) {
+            const int page = page_of(a, b, j >> a.kv.page_shift);
+            if (page >= 0) {
+              off = a.kv.row(page, h, j & mask);
+              if constexpr (BITS != 16) soff = a.kv.scale_row(page, h, j & mask);
+            }
+          }
+          live = off >= 0;
+          for (int it = 0; it < kKeys / kRowsIt; ++it) {
+            const int row = it * kRowsIt + lane / kChunks, c = lane % kChunks;
+            const int64_t ro = __shfl_sync(0xffffffffu, off, row);
+            if (c * 16 < row_bytes) {
+              const int64_t src = ro < 0 ? 0 : ro + c * 16;
+              const uint32_t kd = st + chunk_at<BITS, kChunks, false>(row, c);
+              const uint32_t vd = st + K::kVOff + chunk_at<BITS, kChunks, true>(row, c);
+              const uint32_t n = ro < 0 ? 0u : 8u;
+              if (wide) {
+                cp16(kd, a.kv.k + src, 2 * n);
+                cp16(vd, a.kv.v + src, 2 * n);
+              } else {
+                cp8(kd, a.kv.k + src, n);
+                cp8(vd, a.kv.v + src, n);
+                if (c * 16 + 8 < row_bytes) {
+                  cp8(kd + 8, a.kv.k + src + n, n);
+                  cp8(vd + 8, a.kv.v + src + n, n);
+                }
               }
             }
           }
@@ -317,11 +364,11 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
           const uint32_t sd = st + K::kScOff + static_cast<uint32_t>(lane) * K::kScale;
           constexpr uint32_t kV = kKeys * K::kScale;
           if constexpr (BITS == 8) {
-            cp4(sd, a.kv.k_scale + soff, off < 0 ? 0u : 4u);
-            cp4(sd + kV, a.kv.v_scale + soff, off < 0 ? 0u : 4u);
+            cp4(sd, a.kv.k_scale + soff, live > 0 ? 4u : 0u);
+            cp4(sd + kV, a.kv.v_scale + soff, live > 0 ? 4u : 0u);
           } else {
-            cp8(sd, a.kv.k_scale + soff, off < 0 ? 0u : 8u);
-            cp8(sd + kV, a.kv.v_scale + soff, off < 0 ? 0u : 8u);
+            cp8(sd, a.kv.k_scale + soff, live > 0 ? 8u : 0u);
+            cp8(sd + kV, a.kv.v_scale + soff, live > 0 ? 8u : 0u);
           }
         }
       }
@@ -362,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
           }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = most > 0.f && most < INFINITY ? min(max(ilogbf(most), -126), 126) : 0;
+        const int e = most > 0.f && most < INFINITY ? min(max(ilogbf(most), -100), 100) : 0;
         rf[i] = exp2f(static_cast<float>(e));
       }
     }
@@ -392,14 +439,17 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
           const int d = tig * (DP / 4) + 8 * (ks >> 1) + 2 * (ks & 1);
           qa[ks][i] = q2(i, d, d + 4);
           qa[ks][i + 2] = q2(i, d + 1, d + 5);
+        }
+        if constexpr (BITS != 16) {
           const float2 f = __half22float2(u32_as_h2(qa[ks][i])), g = __half22float2(u32_as_h2(qa[ks][i + 2]));
           qsum[i] += f.x + f.y + g.x + g.y;
         }
       }
     }
-    if constexpr (BITS == 4) {
+    if constexpr (BITS != 16) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if constexpr (K::kRowFactor) rf[i] *= 16777216.f;  // undoes the subnormal codes' 2^-24
         qsum[i] += __shfl_xor_sync(0xffffffffu, qsum[i], 1);
         qsum[i] += __shfl_xor_sync(0xffffffffu, qsum[i], 2);
       }
@@ -417,6 +467,34 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
       const uint32_t st = ring + static_cast<uint32_t>(t % kStages) * K::kStage;
       const int j0 = (p.t0 + tile + t) * K::kUnit + warp * kKeys;
       if (j0 > tile_max) continue;  // nothing here for any row
+      const uint8_t* const stp = smem + (st - smem_u32(smem));
+      if constexpr (BITS != 16) {
+        // lane = key: a = 2^24 s c and z c, with c = scale log2(e); log2 t, 1 / t, y / t.
+        // (bf16: the 2^24 goes with the row factors, whose range takes it)
+        constexpr float kUp = K::kRowFactor ? 1.f : 16777216.f, kDown = K::kRowFactor ? 5.9604644775390625e-8f : 1.f;
+        const float* ksc = reinterpret_cast<const float*>(stp + K::kScOff);
+        const float* vsc = ksc + kKeys * K::kScale / 4;
+        float step, base, vstep, vbase = 0.f;
+        if constexpr (BITS == 8) {
+          step = ksc[lane];
+          base = -128.f * step;
+          vstep = vsc[lane];
+        } else {
+          const float2 kk = reinterpret_cast<const float2*>(ksc)[lane], vv = reinterpret_cast<const float2*>(vsc)[lane];
+          step = kk.x;
+          base = kk.y;
+          vstep = vv.x;
+          vbase = fmaf(8.f, vv.x, vv.y);
+        }
+        vstep = vstep < kMinScale ? kMinScale : vstep;  // a step of zero; a NaN stays
+        const float lv = lg2(vstep), inv = ex2(-lv);
+        prep[lane] = step * cs * kUp;
+        prep[kKeys + lane] = lv;
+        prep[2 * kKeys + lane] = inv;
+        prep[3 * kKeys + lane] = base * cs * kDown;
+        // (the rounded quotient: codes and base nearly cancel where a value is near zero)
+        if constexpr (BITS == 4) prep[4 * kKeys + lane] = vbase / vstep;
+      }
       float s[kNt][4];
 #pragma unroll
       for (int i = 0; i < kNt; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
@@ -431,65 +509,63 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
       } else {
         constexpr int kBytes = DP * BITS / 32;          // of a row, a thread
         constexpr int kWords = kBytes >= 16 ? 4 : 2;    // a load
+        using Words = std::conditional_t<kWords == 4, uint4, uint2>;
 #pragma unroll
         for (int i = 0; i < kNt; ++i) {
 #pragma unroll
           for (int n = 0; n < kBytes / (4 * kWords); ++n) {
             const int byte = tig * kBytes + n * 4 * kWords;
-            uint32_t w[kWords];
-            lds_words<kWords>(st + chunk_at<BITS, kChunks, false>(8 * i + gid, byte >> 4) + (byte & 15), w);
+            const Words ww = *reinterpret_cast<const Words*>(stp + chunk_at<BITS, kChunks, false>(8 * i + gid, byte >> 4) + (byte & 15));
+            uint32_t w[4];
+            w[0] = ww.x;
+            w[1] = ww.y;
+            if constexpr (kWords == 4) {
+              w[2] = ww.z;
+              w[3] = ww.w;
+            }
 #pragma unroll
             for (int e = 0; e < kWords; ++e) {
+              const int ks = n * kWords + e;
               if constexpr (BITS == 8) {
                 const uint32_t x = w[e] ^ 0x80808080u;
-                mma<C>(s[i], qa[n * kWords + e], codes8(__byte_perm(x, 0x64646464u, 0x4140)),
-                       codes8(__byte_perm(x, 0x64646464u, 0x4342)));
+                mma<C>(s[i], qa[ks], __byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342));
               } else {
-                mma<C>(s[i], qa[2 * (n * kWords + e)], codes4(w[e], 0), codes4(w[e], 1));
-                mma<C>(s[i], qa[2 * (n * kWords + e) + 1], codes4(w[e], 2), codes4(w[e], 3));
+                constexpr uint32_t kLow = 0x000f000fu;
+                mma<C>(s[i], qa[2 * ks], w[e] & kLow, (w[e] >> 4) & kLow);
+                mma<C>(s[i], qa[2 * ks + 1], (w[e] >> 8) & kLow, (w[e] >> 12) & kLow);
               }
             }
           }
         }
       }
       // scores, in powers of two
-      float inv[kNt][2], zr[kNt][2];
+      float2 inv[kNt], zr[kNt];
       if constexpr (BITS == 16) {
 #pragma unroll
         for (int i = 0; i < kNt; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[i][e] *= cs;
       } else {
-        const float* ksc = reinterpret_cast<const float*>(smem + (st - smem_u32(smem)) + K::kScOff);
-        const float* vsc = ksc + kKeys * K::kScale / 4;
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < kNt; ++i)
+        for (int i = 0; i < kNt; ++i) {
+          const int j = 8 * i + 2 * tig;
+          const float2 aj = *reinterpret_cast<const float2*>(prep + j);
+          const float2 lv = *reinterpret_cast<const float2*>(prep + kKeys + j);
+          const float2 zj = *reinterpret_cast<const float2*>(prep + 3 * kKeys + j);
+          inv[i] = *reinterpret_cast<const float2*>(prep + 2 * kKeys + j);
+          if constexpr (BITS == 4) zr[i] = *reinterpret_cast<const float2*>(prep + 4 * kKeys + j);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = 8 * i + 2 * tig + e;
-            float ks_, kz = 0.f, vs_, vz = 0.f;
-            if constexpr (BITS == 8) {
-              ks_ = ksc[j];
-              vs_ = vsc[j];
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (K::kRowFactor) {
+              s[i][2 * r] = fmaf(fmaf(qsum[r], zj.x, s[i][2 * r] * aj.x), rf[r], lv.x);
+              s[i][2 * r + 1] = fmaf(fmaf(qsum[r], zj.y, s[i][2 * r + 1] * aj.y), rf[r], lv.y);
             } else {
-              const float2 kk = reinterpret_cast<const float2*>(ksc)[j], vv = reinterpret_cast<const float2*>(vsc)[j];
-              ks_ = kk.x;
-              kz = fmaf(8.f, kk.x, kk.y);
-              vs_ = vv.x;
-              vz = fmaf(8.f, vv.x, vv.y);
-            }
-            vs_ = vs_ < kMinScale ? kMinScale : vs_;  // a step of zero; a NaN stays
-            const float lv = lg2(vs_);
-            inv[i][e] = 1.f / vs_;
-            zr[i][e] = vz * inv[i][e];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float x = s[i][e + 2 * r] * ks_;
-              if constexpr (BITS == 4) x = fmaf(qsum[r], kz, x);
-              if constexpr (K::kRowFactor) x *= rf[r];
-              s[i][e + 2 * r] = fmaf(x, cs, lv);
+              s[i][2 * r] = fmaf(s[i][2 * r], aj.x, fmaf(qsum[r], zj.x, lv.x));
+              s[i][2 * r + 1] = fmaf(s[i][2 * r + 1], aj.y, fmaf(qsum[r], zj.y, lv.y));
             }
           }
+        }
       }
       const bool full = j0 + kKeys - 1 <= tile_min && (a.window <= 0 || j0 > tile_max - a.window);
       if (!full) {
@@ -541,7 +617,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
           } else {
             // what a row does not see may have any step: it stays out of the sums
             const bool in = full || s[i][e] != -INFINITY;
-            l[r] += in ? w[e] * inv[i][e & 1] : 0.f;
+            l[r] += in ? w[e] * (e & 1 ? inv[i].y : inv[i].x) : 0.f;
           }
         }
 #pragma unroll
@@ -552,8 +628,8 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
             // the rounded weights, so that their rounding scales with the value and not
             // with the code's distance from 8
             const float2 f = unpack2<C>(pair);
-            zacc[r] += full || s[i][2 * r] != -INFINITY ? f.x * zr[i][0] : 0.f;
-            zacc[r] += full || s[i][2 * r + 1] != -INFINITY ? f.y * zr[i][1] : 0.f;
+            zacc[r] += full || s[i][2 * r] != -INFINITY ? f.x * zr[i].x : 0.f;
+            zacc[r] += full || s[i][2 * r + 1] != -INFINITY ? f.y * zr[i].y : 0.f;
           }
         }
       }
@@ -562,7 +638,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
         if (!full) {
           for (int i = lane; i < kKeys * kChunks; i += 32) {
             if (i % kChunks * 16 >= row_bytes) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(smem + (st - smem_u32(smem)) + K::kVOff +
+            const uint4 v = *reinterpret_cast<const uint4*>(stp + K::kVOff +
                                                             chunk_at<BITS, kChunks, true>(i / kChunks, i % kChunks));
             const uint32_t ws[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -601,7 +677,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
               for (int e = 0; e < 2; ++e) {
                 const int d = 8 * i + 2 * tig + e;
                 if (d >= D) continue;
-                const float v = to_f32(*reinterpret_cast<const T*>(smem + (st - smem_u32(smem)) + K::kVOff +
+                const float v = to_f32(*reinterpret_cast<const T*>(stp + K::kVOff +
                                                                    chunk_at<BITS, kChunks, true>(j, d >> 3) + (d & 7) * 2));
                 if (sees[0]) o[i][e] = fmaf(w[0], v, o[i][e]);
                 if (sees[1]) o[i][2 + e] = fmaf(w[1], v, o[i][2 + e]);
@@ -617,27 +693,30 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnArgs a, const P
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int row = kk * 16 + 2 * tig + (e & 1) + (e >> 1) * 8;
-              w[e] = lds32(st + K::kVOff + chunk_at<BITS, kChunks, true>(row, 2 * n + (gid >> 2)) + (gid & 3) * 4);
+              w[e] = *reinterpret_cast<const uint32_t*>(stp + K::kVOff +
+                                                        chunk_at<BITS, kChunks, true>(row, 2 * n + (gid >> 2)) + (gid & 3) * 4);
             }
             if constexpr (BITS == 8) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
+              // bytes 0 and 1, then 2 and 3, of two rows side by side
+              const uint32_t g[2][2] = {{__byte_perm(w[0], w[1], 0x5140), __byte_perm(w[2], w[3], 0x5140)},
+                                        {__byte_perm(w[0], w[1], 0x7362), __byte_perm(w[2], w[3], 0x7362)}};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const uint32_t sel = static_cast<uint32_t>(j | (4 + j) << 8);
-                auto pick = [&](uint32_t x, uint32_t y) {
-                  const uint32_t g = __byte_perm(x, y, (sel & 15u) | (sel >> 8) << 8);
-                  return codes8((g & 0x00ff00ffu) | 0x64006400u);
-                };
-                mma<C>(o[4 * n + j], pa[kk], pick(w[0], w[1]), pick(w[2], w[3]));
+                const uint32_t sel = j & 1 ? 0x4342u : 0x4140u;
+                mma<C>(o[4 * n + j], pa[kk], signed8(__byte_perm(g[j >> 1][0], 0x64646464u, sel)),
+                       signed8(__byte_perm(g[j >> 1][1], 0x64646464u, sel)));
               }
             } else {
-              const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5410), hi0 = __byte_perm(w[0], w[1], 0x7632);
-              const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5410), hi1 = __byte_perm(w[2], w[3], 0x7632);
+              // codes 0..3, then 4..7, of two rows
+              const uint32_t g[2][2] = {{__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410)},
+                                        {__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632)}};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                mma<C>(o[8 * n + j], pa[kk], codes4(lo0, j), codes4(lo1, j));
-                mma<C>(o[8 * n + 4 + j], pa[kk], codes4(hi0, j), codes4(hi1, j));
+                const uint32_t x = g[j >> 1][0] >> (j & 1 ? 8 : 0), y = g[j >> 1][1] >> (j & 1 ? 8 : 0);
+                mma<C>(o[8 * n + 2 * j], pa[kk], signed4<0>(x), signed4<0>(y));
+                mma<C>(o[8 * n + 2 * j + 1], pa[kk], signed4<1>(x), signed4<1>(y));
               }
             }
           }

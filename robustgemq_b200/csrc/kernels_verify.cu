@@ -27,6 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxParts = 32;   // one lane a part where the parts are joined
 constexpr int kMaxRows = 64;    // drafts + 1
+constexpr int kPickBlocks = 4;  // of the second kernel, resident on an SM
 
 struct VerifyArgs {
   const void* logits;          // [B][n + 1][V]
@@ -144,9 +145,10 @@ __device__ __forceinline__ Stat row_stat(const L* row, int j0, int j1, float f) 
 __device__ __forceinline__ float slope(float t) { return kLog2e / (t == 0.f ? 1.f : t); }
 
 template <typename L>
-__global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) k_verify_stats(const VerifyArgs a) {
   __shared__ Stat s_warp[kWarps];
   grid_dep_wait();
+  grid_dep_launch();  // the pick's blocks may come up in the tail of this kernel
   const int part = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
   if (part == 0 && i == 0 && threadIdx.x == 0) {
     a.best[2 * b] = a.best[2 * b + 1] = 0ull;
@@ -217,7 +219,7 @@ __device__ __forceinline__ Race run_race(const L* lr, const Q* qr, int x_r, cons
 }
 
 template <typename L, typename Q>
-__global__ void __launch_bounds__(kThreads) k_verify_pick(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, kPickBlocks) k_verify_pick(const VerifyArgs a) {
   __shared__ Stat s_row[kMaxRows];
   __shared__ unsigned long long s_best[2][kWarps];
   __shared__ bool s_last;
@@ -314,14 +316,17 @@ __global__ void __launch_bounds__(kThreads) k_verify_pick(const VerifyArgs a) {
   if (lane == 0) a.accepted[b] = r;
 }
 
-// Parts of a row for `rows` of them: blocks for four on each SM, at least one step of
-// 8 * kThreads values each, at most `most`.
-int parts_of(int64_t rows, int V, int most) {
-  const int64_t want = (4 * device_sm_count() + rows - 1) / rows;
+// Parts of a row for `rows` of them: at least one step of 8 * kThreads values each.
+// Statistics: sixteen blocks an SM, so that the last round of them is a small share. The
+// race: one round of resident blocks, since every block first repeats the decisions.
+int parts_of(int64_t rows, int V, int64_t blocks, int most) {
+  const int64_t want = std::max<int64_t>(1, blocks / rows);
   const int64_t steps = (V + 8 * kThreads - 1) / (8 * kThreads);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, steps, most})));
+  return static_cast<int>(std::min<int64_t>({want, steps, most}));
 }
-int stat_parts(int B, int n, int V) { return parts_of(static_cast<int64_t>(B) * (n + 1), V, kMaxParts); }
+int stat_parts(int B, int n, int V) {
+  return parts_of(static_cast<int64_t>(B) * (n + 1), V, 16 * device_sm_count(), kMaxParts);
+}
 // Values of a part: a multiple of 8, so that parts of an aligned row are aligned.
 int part_length(int V, int parts) { return ((V + parts - 1) / parts + 7) / 8 * 8; }
 
@@ -352,7 +357,7 @@ cudaError_t launch_verify(const gemq_verify_t& v, int B, int n, int V, void* wor
   a.V = V;
   a.parts = stat_parts(B, n, V);
   a.part_len = part_length(V, a.parts);
-  const int races = parts_of(B, V, 1024);
+  const int races = parts_of(B, V, kPickBlocks * device_sm_count(), 1024);
   a.race_len = part_length(V, races);
   char* w = static_cast<char*>(workspace);
   a.stats = reinterpret_cast<float4*>(w);

@@ -18,22 +18,27 @@ namespace gemq {
 // times any sequence length inside fp32.
 constexpr float kMinScale = 5.421010862427522e-20f;  // 2^-64
 
-// gemq_kv_cache_t as the kernels take it. Strides: bytes between pages, heads and
-// tokens of the codes; floats between those of the scales.
+// gemq_kv_cache_t as the kernels take it. Strides between pages, heads and tokens: of the
+// codes in units of 8 bytes, of the scales in floats; below 2^31 each, so that a row's
+// address takes three 32 x 32 -> 64 bit multiply-adds.
 struct KvDev {
   uint8_t* k;
   uint8_t* v;
   float* k_scale;
   float* v_scale;
-  int64_t page_stride, head_stride, token_stride;
-  int64_t scale_page_stride, scale_head_stride, scale_token_stride;
+  uint32_t page_stride, head_stride, token_stride;
+  uint32_t scale_page_stride, scale_head_stride, scale_token_stride;
   int num_pages, kv_heads, page_shift, head_dim;
 
   __device__ __forceinline__ int64_t row(int page, int head, int off) const {
-    return page * page_stride + head * head_stride + off * token_stride;
+    return static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_stride +
+                                 static_cast<uint64_t>(static_cast<uint32_t>(head)) * head_stride +
+                                 static_cast<uint64_t>(static_cast<uint32_t>(off)) * token_stride) << 3);
   }
   __device__ __forceinline__ int64_t scale_row(int page, int head, int off) const {
-    return page * scale_page_stride + head * scale_head_stride + off * scale_token_stride;
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * scale_page_stride +
+                                static_cast<uint64_t>(static_cast<uint32_t>(head)) * scale_head_stride +
+                                static_cast<uint64_t>(static_cast<uint32_t>(off)) * scale_token_stride);
   }
 };
 

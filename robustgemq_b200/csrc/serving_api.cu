@@ -67,6 +67,9 @@ int check_cache(const gemq_kv_cache_t* c) {
       ok = ok && c->scale_strides[i] >= 0 && (c->bits == 8 || c->scale_strides[i] % 2 == 0);
   }
   if (!ok) return fail(GEMQ_ERR_UNSUPPORTED, "cache: k, v, the scales and the strides must be aligned (16 bytes a row)");
+  for (int i = 0; i < 3; ++i)
+    if (c->strides[i] / 8 > INT32_MAX || (c->bits != 16 && c->scale_strides[i] > INT32_MAX))
+      return fail(GEMQ_ERR_UNSUPPORTED, "cache: a stride of 2^34 bytes or more");
   return GEMQ_OK;
 }
 
@@ -76,12 +79,12 @@ KvDev to_dev(const gemq_kv_cache_t& c) {
   d.v = static_cast<uint8_t*>(c.v);
   d.k_scale = c.k_scale;
   d.v_scale = c.v_scale;
-  d.page_stride = c.strides[0];
-  d.head_stride = c.strides[1];
-  d.token_stride = c.strides[2];
-  d.scale_page_stride = c.scale_strides[0];
-  d.scale_head_stride = c.scale_strides[1];
-  d.scale_token_stride = c.scale_strides[2];
+  d.page_stride = static_cast<uint32_t>(c.strides[0] / 8);
+  d.head_stride = static_cast<uint32_t>(c.strides[1] / 8);
+  d.token_stride = static_cast<uint32_t>(c.strides[2] / 8);
+  d.scale_page_stride = c.bits == 16 ? 0u : static_cast<uint32_t>(c.scale_strides[0]);
+  d.scale_head_stride = c.bits == 16 ? 0u : static_cast<uint32_t>(c.scale_strides[1]);
+  d.scale_token_stride = c.bits == 16 ? 0u : static_cast<uint32_t>(c.scale_strides[2]);
   d.num_pages = c.num_pages;
   d.kv_heads = c.kv_heads;
   d.page_shift = 0;
