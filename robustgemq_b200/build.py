@@ -21,7 +21,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libgemq_b200.so"
 SOURCES = ["gemq_api.cu", "kernels_misc.cu", "kernels_route.cu", "kernels_decode.cu", "kernels_tc.cu",
-           "kernels_tcd.cu", "kernels_simt.cu", "kernels_cache.cu", "kernels_attn.cu", "kernels_verify.cu",
+           "kernels_tcd.cu", "kernels_simt.cu", "kernels_cache.cu", "kernels_attn.cu", "kernels_attn_tc.cu", "kernels_verify.cu",
            "serving_api.cu"]
 HEADERS = ["gemq_common.cuh", "gemq_internal.h", "tc_work.cuh", "kperm.cuh", "paged.cuh", "attn_rows.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1046,13 +1046,22 @@ int most_rows(const AttnArgs& a, int max_q_len) {
   return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(max_q_len) * a.group, 1 << 20));
 }
 
+// More rows a KV head than kFewRows go to the tensor-memory kernel.
+constexpr int kFewRows = 32;
+bool takes_many(const AttnArgs& a, int max_q_len) {
+  return most_rows(a, max_q_len) > kFewRows && a.kv.head_dim <= 128;
+}
+
 }  // namespace
 
-size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int) {
+size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len) {
+  if (takes_many(a, max_q_len)) return many_workspace(a, bits, bf16, max_q_len, max_kv_len);
   return with_few(bits, bf16, a.kv.head_dim, most_rows(a, max_q_len), [&](auto k) { return decltype(k)::workspace(); });
 }
 
-cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int, void* workspace, cudaStream_t s) {
+cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
+                             cudaStream_t s) {
+  if (takes_many(a, max_q_len)) return launch_many(a, bits, bf16, max_q_len, max_kv_len, workspace, s);
   const int rows = most_rows(a, max_q_len);
   return with_few(bits, bf16, a.kv.head_dim, rows, [&](auto k) { return decltype(k)::launch(a, rows, workspace, s); });
 }

@@ -156,6 +156,10 @@ cudaError_t launch_cache_read(const KvDev& c, int bits, bool bf16, const int64_t
 size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len);
 cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
                              cudaStream_t s);
+// (kernels_attn_tc.cu: many rows a KV head; head_dim at most 128)
+size_t many_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len);
+cudaError_t launch_many(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
+                        cudaStream_t s);
 size_t verify_workspace(int B, int n, int V);
 cudaError_t launch_verify(const gemq_verify_t& v, int B, int n, int V, void* workspace, cudaStream_t s);
 
