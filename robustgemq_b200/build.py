@@ -24,6 +24,8 @@ SOURCES = ["gemq_api.cu", "kernels_misc.cu", "kernels_route.cu", "kernels_decode
            "kernels_tcd.cu", "kernels_simt.cu", "kernels_cache.cu", "kernels_attn.cu", "kernels_attn_tc.cu", "kernels_verify.cu",
            "serving_api.cu"]
 HEADERS = ["gemq_common.cuh", "gemq_internal.h", "tc_work.cuh", "kperm.cuh", "paged.cuh", "attn_rows.cuh"]
+# compiled without relocatable device code: ptxas ignores setmaxnreg with it
+WHOLE = {"kernels_attn_tc.cu"}
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -49,7 +51,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
     objdir = ROOT / "_build"
     objdir.mkdir(exist_ok=True)
     common = [nvcc, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", str(ROOT / "include"),
-              "--expt-relaxed-constexpr", "-rdc=true"]
+              "--expt-relaxed-constexpr"]
     if verbose:
         common += ["-Xptxas", "-v"]
     procs = []
@@ -57,7 +59,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
     for src in SOURCES:
         obj = objdir / (Path(src).stem + ".o")
         objs.append(obj)
-        cmd = common + ["-c", str(CSRC / src), "-o", str(obj)]
+        cmd = common + ([] if src in WHOLE else ["-rdc=true"]) + ["-c", str(CSRC / src), "-o", str(obj)]
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
         if len(procs) >= jobs:
             _wait(procs.pop(0), verbose)

@@ -214,7 +214,9 @@ int gemq_get_device_error(uint32_t* code_out) {
   const uint32_t zero = 0;
   GEMQ_CUDA(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero)), "clear device error");
   GEMQ_CUDA(cudaMemcpyToSymbol(g_device_abort, &zero, sizeof(zero)), "clear device abort");
-  *code_out = v;
+  uint32_t many = 0;
+  GEMQ_CUDA(take_many_error(&many), "read the attention kernel's device error");
+  *code_out = v != 0 ? v : many;
   return GEMQ_OK;
 }
 

@@ -41,8 +41,15 @@ enum DeviceError : uint32_t {
 // g_device_abort: set only when a wait expired; every other pending wait then gives
 // up at once so a broken pipeline drains quickly. Input errors (an out-of-range
 // expert id, a bad bit-width) are recorded without aborting other kernels.
+// A translation unit that is compiled whole (registers can only be moved between warps
+// there) has words of its own, which gemq_get_device_error reads as well.
+#ifdef GEMQ_OWN_ERROR_WORDS
+static __device__ uint32_t g_device_error = 0;
+static __device__ uint32_t g_device_abort = 0;
+#else
 extern __device__ uint32_t g_device_error;
 extern __device__ uint32_t g_device_abort;
+#endif
 
 __device__ __forceinline__ void set_device_error(uint32_t code) { atomicCAS(&g_device_error, 0u, code); }
 __device__ __forceinline__ void set_device_abort(uint32_t code) {

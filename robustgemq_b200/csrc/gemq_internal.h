@@ -204,6 +204,9 @@ cudaError_t launch_decode_combine(const float* part, int splits, int A, int n, c
                                   const float* shared_part, int shared_splits, const uint16_t* residual, uint16_t* out,
                                   cudaStream_t s);
 
+// The error word of kernels_attn_tc.cu (compiled whole, with words of its own), cleared.
+cudaError_t take_many_error(uint32_t* code);
+
 int device_sm_count();
 void set_error(const std::string& msg);
 

@@ -10,11 +10,12 @@
 //               ([key][column]: the N-major form of the B operand)
 // 512 columns of tensor memory hold both chains (2 x 128 for S and P, 2 x up to 128 for
 // O); while one chain's threads take exponentials the tensor cores work for the other.
-// Warps: 0-3 and 4-7 the two chains' softmax (a thread a row), 8 and 9 their MMA issue
-// (a chain's next S overwrites P, so each waits for its own last product; the other
-// warp's go on meanwhile), 10-13 load: 16-bit rows by cp.async, codes by way of registers,
-// unpacked to exact fp16 as they are stored. Pages may have any size: a row's address is
-// looked up per key, a tile ahead.
+// Warps: 0-3 and 4-7 the two chains' softmax (a thread a row, the row's 128 scores in its
+// registers: these warps take 184 each and the others 72), 8 and 9 their MMA issue (a
+// chain's next S overwrites P, so each waits for its own last product; the other warp's go
+// on meanwhile), 12-15 load: 16-bit rows by cp.async, codes by way of registers, unpacked
+// to exact fp16 as they are stored. Pages may have any size: a row's address is looked up
+// per key, a tile ahead.
 //
 // The reference of the exponentials moves only when a row's scores pass it by more than
 // 2^8 (in 16 bits 2^8 is as exact as 1), so that the sums in tensor memory are rarely
@@ -23,6 +24,7 @@
 // Where few tiles there are to fill the machine, each takes part of the keys and
 // k_attn_tiles adds the parts up; with at most 128 rows a KV head both chains take the
 // same rows and every second tile of keys each.
+#define GEMQ_OWN_ERROR_WORDS  // compiled without relocatable device code, for setmaxnreg
 #include <algorithm>
 
 #include "attn_rows.cuh"
@@ -36,9 +38,12 @@ constexpr int kKeys = 128;        // of a tile
 constexpr int kRows = 128;        // of a chain
 constexpr int kSoftWarps = 8;
 constexpr int kMmaWarp = 8;       // and 9
-constexpr int kLoadWarp = 10;
+constexpr int kLoadWarp = 12;
 constexpr int kLoaders = 128;
 constexpr int kThreads = 32 * (kLoadWarp + 4);
+// Registers after the split: 256 x 184 + 256 x 72 = 512 x 128, what the block starts with.
+constexpr int kSoftRegs = 184, kOtherRegs = 72;
+static_assert(256 * (kSoftRegs + kOtherRegs) <= kThreads * 128, "more registers than the block was launched with");
 constexpr float kSlack = 8.f;     // how far a score may pass the reference, in powers of two
 
 template <typename T, int BITS, int DP>
@@ -89,6 +94,68 @@ __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Pairs of fp32.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// The eight K = 16 steps of O += P V, issued from one asm block (their operands are then
+// formed back to back): P 8 columns a step, V 16 keys of 128 bytes.
+__device__ __forceinline__ void umma_pv(uint32_t d, uint32_t p, uint64_t v, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      ".reg .b32 a1, a2, a3, a4, a5, a6, a7;\n\t"
+      ".reg .b64 b1, b2, b3, b4, b5, b6, b7;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.u32 q, 0, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\tadd.u32 a4, %1, 32;\n\t"
+      "add.u32 a5, %1, 40;\n\tadd.u32 a6, %1, 48;\n\tadd.u32 a7, %1, 56;\n\t"
+      "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\tadd.u64 b4, %2, 512;\n\t"
+      "add.u64 b5, %2, 640;\n\tadd.u64 b6, %2, 768;\n\tadd.u64 b7, %2, 896;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a4], b4, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a5], b5, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a6], b6, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a7], b7, %3, q;\n\t}" ::"r"(d),
+      "r"(p), "l"(v), "r"(id), "r"(accumulate)
+      : "memory");
+}
+
+// One arrival for a warp whose lanes have done their part.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // Codes minus their middle as fp16 pairs, exactly (a code under the exponent of 1024, or
@@ -205,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     k1 = t0 + static_cast<int>(static_cast<int64_t>(n) * (span + 1) / ta.spans);
   }
   const int n_tiles = k1 - k0;
-  const float cs = a.scale * kLog2e;
+  const float cs = fabsf(a.scale) * kLog2e;
 
   // which tiles chain i takes: all, or every second one
   const int step = same_rows ? 2 : 1;
@@ -216,16 +283,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   if (threadIdx.x == 0) {
     const int chains = chain_b && !same_rows ? 2 : 1;  // that take each tile
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], kLoaders);
+      mbar_init(&full[s], 4);  // one arrival a warp
       mbar_init(&empty[s], chains);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kRows);
+      mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
-      mbar_init(&prep_full[i], kLoaders);
+      mbar_init(&prep_full[i], 4);
       mbar_init(&prep_empty[i], 4 * chains);  // softmax warps
-      mbar_init(&offs_full[i], kLoaders);
+      mbar_init(&offs_full[i], 4);
       mbar_init(&drain[i], 1);
     }
     fence_barrier_init();
@@ -283,6 +350,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           ws[e] = pack2<__half>(f.x * inv_factor, f.y * inv_factor);
         }
       }
+      if (a.scale < 0.f) {  // (the scores' factor is its magnitude)
+        w.x ^= 0x80008000u;
+        w.y ^= 0x80008000u;
+        w.z ^= 0x80008000u;
+        w.w ^= 0x80008000u;
+      }
       if constexpr (BITS == 4) {
         const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -301,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
 
   bool ok = true;  // no wait of this thread ran out
   if (warp >= kLoadWarp) {
+    regs_down<kOtherRegs>();
     // ---------------------------------------------------------- loads
     const int me = static_cast<int>(threadIdx.x) - kLoadWarp * 32;
     const int mask = (1 << a.kv.page_shift) - 1;
@@ -341,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         }
       }
       fence_proxy_async_smem();
-      mbar_arrive(&full[s]);
+      warp_arrive(&full[s]);
       ++done;
     };
     for (int t = 0; t < n_tiles && ok; ++t) {
@@ -372,8 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           }
         }
       }
-      mbar_arrive(&offs_full[t & 1]);
-      ok = mbar_wait(&offs_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
+      warp_arrive(&offs_full[t & 1]);
+      ok = warp_wait(&offs_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
 #pragma unroll 1
       for (int v = 0; v < 2 && ok; ++v) {
         const int g = 2 * t + v, s = g % kStages;
@@ -402,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
             }
           }
         }
-        if (!mbar_try_wait(smem_u32(&empty[s]), ((g / kStages) & 1) ^ 1u)) {
+        if (!__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&empty[s]), ((g / kStages) & 1) ^ 1u))) {
           if constexpr (BITS == 16) {
             // nothing to issue: hand over what is on its way
             if (done < g) {
@@ -410,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
               hand_over();
             }
           }
-          ok = mbar_wait(&empty[s], ((g / kStages) & 1) ^ 1u, kDevTimeoutAEmpty);
+          ok = warp_wait(&empty[s], ((g / kStages) & 1) ^ 1u, kDevTimeoutAEmpty);
           if (!ok) break;
         }
         if constexpr (BITS == 16) {
@@ -431,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         } else {
           if (v == 0) {
             // the key's factors: a = s c, log2 t, 1 / t, z c, y / t, with c = scale log2(e)
-            ok = mbar_wait(&prep_empty[t & 1], ((t >> 1) & 1) ^ 1u, kDevTimeoutAEmpty);
+            ok = warp_wait(&prep_empty[t & 1], ((t >> 1) & 1) ^ 1u, kDevTimeoutAEmpty);
             if (!ok) break;
             float* const prep = s_prep + (t & 1) * 5 * kKeys;
             const float vstep = vsc.x < kMinScale ? kMinScale : vsc.x;  // a step of zero; a NaN stays
@@ -446,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
               prep[3 * kKeys + me] = fmaf(8.f, ksc.x, ksc.y) * cs;
               prep[4 * kKeys + me] = fabsf(zr) < INFINITY ? zr : 0.f;
             }
-            mbar_arrive(&prep_full[t & 1]);
+            warp_arrive(&prep_full[t & 1]);
           }
           if (c * 16 < row_bytes) {
 #pragma unroll
@@ -473,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
             }
           }
           fence_proxy_async_smem();
-          mbar_arrive(&full[s]);
+          warp_arrive(&full[s]);
         }
       }
     }
@@ -484,8 +558,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     }
   } else if (warp >= kMmaWarp) {
     // ---------------------------------------------------------- products of one chain
+    regs_down<kOtherRegs>();
     const int i = warp - kMmaWarp;
-    if (i == 0 || chain_b) {
+    if (i == 0 || (i == 1 && chain_b)) {
       const uint32_t s_col = tmem + i * 128, o_col = tmem + 256 + i * DP;
       const uint32_t id_s = idesc(K::kType, kKeys, false), id_o = idesc(K::kType, D, true);
       const uint32_t q_addr = smem_u32(smem + K::kQOff + i * K::kTile);
@@ -500,7 +575,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         tc_fence_after();
         const uint32_t k_addr = smem_u32(smem + K::kRingOff + (gk % kStages) * K::kTile);
         if (elect_one()) {
-          for (int k = 0; k < ks; ++k) {
+          int k = 0;
+          for (; k + 4 <= ks; k += 4)
+            umma_f16_k64(s_col, sdesc_sw128(q_addr + (k >> 2) * K::kPanel), sdesc_sw128(k_addr + (k >> 2) * K::kPanel), id_s, k > 0);
+          for (; k < ks; ++k) {
             const uint32_t at = (k >> 2) * K::kPanel + (k & 3) * 32;
             umma_f16(s_col, sdesc_sw128(q_addr + at), sdesc_sw128(k_addr + at), id_s, k > 0);
           }
@@ -514,9 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         tc_fence_after();
         const uint32_t v_addr = smem_u32(smem + K::kRingOff + (gv % kStages) * K::kTile);
         if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_f16_ts(o_col, s_col + 8 * k, sdesc_v(v_addr + k * 2048, K::kPanel), id_o, n > 0 || k > 0);
+          umma_pv(o_col, s_col, sdesc_v(v_addr, K::kPanel), id_o, n > 0);
           umma_commit(&o_done[i]);
           umma_commit(&empty[gv % kStages]);
         }
@@ -526,7 +602,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       __syncwarp();
       mbar_wait_drain(&drain[i], 0);
     }
-  } else if (chain == 0 || chain_b) {
+  } else {
+    regs_up<kSoftRegs>();
+    if (chain == 0 || chain_b) {
     // ---------------------------------------------------------- softmax: a thread a row
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp
     const uint32_t s_col = tmem + lanes + chain * 128, o_col = tmem + lanes + 256 + chain * DP;
@@ -544,86 +622,51 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       ok = ok && warp_wait(&s_full[chain], n & 1, kDevTimeoutAccFull);
       if (!ok) break;
       tc_fence_after();
-      uint32_t p[kKeys / 2];
-      float top, lt, zt;
-      // one pass over S: weights by the present reference, and the row's maximum
-      auto pass = [&](float rr) {
-        top = -INFINITY;
-        lt = zt = 0.f;
+      uint32_t s[kKeys];
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
-          uint32_t raw[32];
-          tmem_ld32(s_col + 32 * c, raw);
-          tmem_ld_wait();
+      for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(s_col + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
+      tmem_ld_wait();
+      auto sf = [&](int j) { return __uint_as_float(s[j]); };
+      if constexpr (BITS != 16) {
+        // scores of codes, with the values' steps in them
+        const F2 qs2 = f2(qsum, qsum), rf2 = f2(rf, rf);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float x[4], iv[4], zr[4];
-            if constexpr (BITS == 16) {
+        for (int j = 0; j < kKeys; j += 4) {
+          const float4 aj = *reinterpret_cast<const float4*>(prep + j);
+          const float4 lv = *reinterpret_cast<const float4*>(prep + kKeys + j);
+          float4 zj = make_float4(0.f, 0.f, 0.f, 0.f);
+          if constexpr (BITS == 4) zj = *reinterpret_cast<const float4*>(prep + 3 * kKeys + j);
 #pragma unroll
-              for (int f = 0; f < 4; ++f) x[f] = __uint_as_float(raw[e + f]) * cs;
-            } else {
-              const int j = 32 * c + e;
-              const float4 aj = *reinterpret_cast<const float4*>(prep + j);
-              const float4 lv = *reinterpret_cast<const float4*>(prep + kKeys + j);
-              const float4 in = *reinterpret_cast<const float4*>(prep + 2 * kKeys + j);
-              const float as[4] = {aj.x, aj.y, aj.z, aj.w}, ls[4] = {lv.x, lv.y, lv.z, lv.w};
-              iv[0] = in.x, iv[1] = in.y, iv[2] = in.z, iv[3] = in.w;
-              float zs[4] = {0.f, 0.f, 0.f, 0.f};
-              if constexpr (BITS == 4) {
-                const float4 zj = *reinterpret_cast<const float4*>(prep + 3 * kKeys + j);
-                const float4 zv = *reinterpret_cast<const float4*>(prep + 4 * kKeys + j);
-                zs[0] = zj.x, zs[1] = zj.y, zs[2] = zj.z, zs[3] = zj.w;
-                zr[0] = zv.x, zr[1] = zv.y, zr[2] = zv.z, zr[3] = zv.w;
-              }
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                const float s = __uint_as_float(raw[e + f]);
-                if constexpr (K::kRowFactor) {
-                  x[f] = fmaf(BITS == 4 ? fmaf(qsum, zs[f], s * as[f]) : s * as[f], rf, ls[f]);
-                } else {
-                  x[f] = fmaf(s, as[f], BITS == 4 ? fmaf(qsum, zs[f], ls[f]) : ls[f]);
-                }
-              }
-            }
-            if (!whole) {
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                const int j = j0 + 32 * c + e + f;
-                if (j > last || j < from) x[f] = -INFINITY;
-              }
-            }
-            float w[4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              top = fmaxf(top, x[f]);
-              w[f] = ex2(x[f] - rr);
-            }
-            const uint32_t p0 = pack2<C>(w[0], w[1]), p1 = pack2<C>(w[2], w[3]);
-            p[16 * c + e / 2] = p0;
-            p[16 * c + e / 2 + 1] = p1;
-            if constexpr (BITS == 16) {
-              lt += (w[0] + w[1]) + (w[2] + w[3]);
-            } else {
-#pragma unroll
-              for (int f = 0; f < 4; ++f) lt = fmaf(w[f], iv[f], lt);
-              if constexpr (BITS == 4) {
-                const float2 f0 = unpack2<C>(p0), f1 = unpack2<C>(p1);
-                zt = fmaf(f0.x, zr[0], zt);
-                zt = fmaf(f0.y, zr[1], zt);
-                zt = fmaf(f1.x, zr[2], zt);
-                zt = fmaf(f1.y, zr[3], zt);
-              }
-            }
+          for (int e = 0; e < 2; ++e) {
+            const F2 a2 = e ? f2(aj.z, aj.w) : f2(aj.x, aj.y), l2 = e ? f2(lv.z, lv.w) : f2(lv.x, lv.y);
+            const F2 z2 = e ? f2(zj.z, zj.w) : f2(zj.x, zj.y), s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
+            F2 x;
+            if constexpr (K::kRowFactor) x = fma2(BITS == 4 ? fma2(s2, a2, mul2(qs2, z2)) : mul2(s2, a2), rf2, l2);
+            else x = fma2(s2, a2, BITS == 4 ? fma2(qs2, z2, l2) : l2);
+            float x0, x1;
+            split(x, x0, x1);
+            s[j + 2 * e] = __float_as_uint(x0);
+            s[j + 2 * e + 1] = __float_as_uint(x1);
           }
         }
-      };
-      pass(ref == -INFINITY ? 0.f : ref);
-      // (a row whose reference is not set yet, or is left behind, takes its maximum)
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+          if (j0 + j > last || j0 + j < from) s[j] = 0xff800000u;  // -inf
+      }
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kKeys; j += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tops[e] = fmaxf(fmaxf(tops[e], sf(j + 2 * e)), sf(j + 2 * e + 1));
+      // (cs is not negative: the queries carry its sign)
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * (BITS == 16 ? cs : 1.f);
+      // a row whose reference is not set yet, or is left behind, takes its maximum
       const bool behind = ref == -INFINITY ? top > -INFINITY : top > ref + kSlack;
       if (__any_sync(0xffffffffu, behind)) {
         const float now = behind ? top : ref;
         const float keep = now == -INFINITY ? 1.f : ex2(ref - now);  // ref = -inf: 0
-        pass(now == -INFINITY ? 0.f : now);
         l *= keep;
         zacc *= keep;
         ref = now;
@@ -642,22 +685,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           }
         }
       }
-      l += lt;
-      zacc += zt;
-      if constexpr (BITS != 16) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&prep_empty[t & 1]);
-      }
+      const float base = ref == -INFINITY ? 0.f : ref;
+      const F2 base2 = f2(-base, -base), cs2 = f2(cs, cs);
+      F2 lt[2] = {f2(l, 0.f), f2(0.f, 0.f)}, zt = f2(zacc, 0.f);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t half[32];
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) half[e] = p[32 * c + e];
-        tmem_st32(s_col + 32 * c, half);
+        for (int i = 0; i < 32; i += 2) {
+          const int j = 64 * half + 2 * i;
+          float4 iv, zr;
+          if constexpr (BITS != 16) iv = *reinterpret_cast<const float4*>(prep + 2 * kKeys + j);
+          if constexpr (BITS == 4) zr = *reinterpret_cast<const float4*>(prep + 4 * kKeys + j);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const F2 s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
+            float y0, y1;
+            split(BITS == 16 ? fma2(s2, cs2, base2) : add2(s2, base2), y0, y1);
+            const float w0 = ex2(y0), w1 = ex2(y1);
+            p[i + e] = pack2<C>(w0, w1);
+            if constexpr (BITS == 16) {
+              lt[e] = add2(lt[e], f2(w0, w1));
+            } else {
+              lt[e] = fma2(f2(w0, w1), e ? f2(iv.z, iv.w) : f2(iv.x, iv.y), lt[e]);
+              if constexpr (BITS == 4) {
+                // the rounded weights, so that their rounding scales with the value and
+                // not with the code's distance from 8
+                const float2 f = unpack2<C>(p[i + e]);
+                zt = fma2(f2(f.x, f.y), e ? f2(zr.z, zr.w) : f2(zr.x, zr.y), zt);
+              }
+            }
+          }
+        }
+        tmem_st32(s_col + 32 * half, p);
       }
+      {
+        float x0, x1, y0, y1;
+        split(lt[0], x0, x1);
+        split(lt[1], y0, y1);
+        l = (x0 + x1) + (y0 + y1);
+        split(zt, x0, x1);
+        zacc = x0 + x1;
+      }
+      if constexpr (BITS != 16) warp_arrive(&prep_empty[t & 1]);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[chain]);
+      warp_arrive(&p_full[chain]);
     }
     // ---------------------------------------------------------- rows out
     if (ok && n > 0) ok = warp_wait(&o_done[chain], (n - 1) & 1, kDevTimeoutAccFull);
@@ -702,6 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         }
       }
     }
+  }
   }
   tc_fence_before();
   __syncthreads();
@@ -830,6 +904,14 @@ auto with_many(int bits, bool bf16, int head_dim, F&& f) {
 }
 
 }  // namespace
+
+cudaError_t take_many_error(uint32_t* code) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
+  const uint32_t zero = 0;
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_device_abort, &zero, sizeof(zero));
+  return e;
+}
 
 size_t many_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len) {
   const Plan p = plan(a, max_q_len, max_kv_len);
