@@ -709,10 +709,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, BITS, DP, NR>::kBlocks) k_att
               l[r][1] = fmaf(w1, inv[i][hi], l[r][1]);
               if constexpr (BITS == 4) {
                 // the rounded weights, so that their rounding scales with the value and
-                // not with the code's distance from 8
+                // not with the code's distance from 8 (but below fp16's normal range,
+                // where a row of equal values comes with its tiny step, the weight itself)
                 const float2 f = unpack2<C>(pair);
-                zacc[r][0] = fmaf(f.x, zr[i][hi], zacc[r][0]);
-                zacc[r][1] = fmaf(f.y, zr[i][hi], zacc[r][1]);
+                zacc[r][0] = fmaf(w0 < kHalfMin ? w0 : f.x, zr[i][hi], zacc[r][0]);
+                zacc[r][1] = fmaf(w1 < kHalfMin ? w1 : f.y, zr[i][hi], zacc[r][1]);
               }
             }
           }

@@ -3,19 +3,25 @@
 //
 // One block takes 256 rows (tokens x query heads that share a KV head) as two tiles of
 // 128, each a chain of its own, over all the keys they see (or one of several spans of
-// them), 128 at a time:
+// them), 80 at a time (128 with at most 64 columns):
 //   S = Q K^T   tcgen05.mma, Q and K from shared memory, S fp32 in tensor memory
-//   P = 2^(S - ref) in 16 bits, back into S's columns
+//   P = 2^(S - ref) in 16 bits, in tensor memory
 //   O += P V    tcgen05.mma, P from tensor memory, V from shared memory as it is stored
 //               ([key][column]: the N-major form of the B operand)
-// 512 columns of tensor memory hold both chains (2 x 128 for S and P, 2 x up to 128 for
-// O); while one chain's threads take exponentials the tensor cores work for the other.
-// Warps: 0-3 and 4-7 the two chains' softmax (a thread a row, the row's 128 scores in its
-// registers: these warps take 184 each and the others 72), 8 and 9 their MMA issue (a
-// chain's next S overwrites P, so each waits for its own last product; the other warp's go
-// on meanwhile), 12-15 load: 16-bit rows by cp.async, codes by way of registers, unpacked
-// to exact fp16 as they are stored. Pages may have any size: a row's address is looked up
-// per key, a tile ahead.
+// The tile is what lets S, P and O of both chains stand side by side in the 512 columns
+// (2 x (80 + 40 + 128)): a chain's next S is formed as soon as its threads have the last
+// one in registers, and both products run under the exponentials. (With 128 keys P had to
+// overwrite S, and each tile's exponentials waited for two products in a row: 4750 cycles
+// a tile with the chains left to themselves, 4250 with the exponentials in turns.)
+// Warps: 0-3 and 4-7 the two chains' softmax (a thread a row, the row's scores in its
+// registers: these warps take 184 each and the others 72), 8 and 9 their MMA issue, 12-15
+// load: 16-bit rows by TMA, codes by way of registers, unpacked to exact fp16 as they are
+// stored.
+//
+// Codes: the steps of values enter as w'_j = w_j t_j / 2^E with one E a block, the
+// largest exponent of a step so far, and o = 2^E sum_j w'_j (d_j + y_j / t_j) / sum_j w_j.
+// A key then has two factors (four at 4 bits) that its 256 rows read from shared memory;
+// the form of kernels_attn.cu has one more, and their delivery is this kernel's bound.
 //
 // The reference of the exponentials moves only when a row's scores pass it by more than
 // 2^8 (in 16 bits 2^8 is as exact as 1), so that the sums in tensor memory are rarely
@@ -25,6 +31,8 @@
 // k_attn_tiles adds the parts up; with at most 128 rows a KV head both chains take the
 // same rows and every second tile of keys each.
 #define GEMQ_OWN_ERROR_WORDS  // compiled without relocatable device code, for setmaxnreg
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 
 #include "attn_rows.cuh"
@@ -34,7 +42,6 @@ namespace gemq {
 
 namespace {
 
-constexpr int kKeys = 128;        // of a tile
 constexpr int kRows = 128;        // of a chain
 constexpr int kSoftWarps = 8;
 constexpr int kMmaWarp = 8;       // and 9
@@ -48,24 +55,31 @@ constexpr float kSlack = 8.f;     // how far a score may pass the reference, in 
 
 template <typename T, int BITS, int DP>
 struct Tc {
-  static constexpr int kPanels = DP / 64;          // of 64 columns (128 bytes) each
-  static constexpr int kPanel = kKeys * 128;       // bytes
-  static constexpr int kTile = kPanels * kPanel;   // Q tile, K tile, V tile
-  static constexpr int kStages = 4;                // K and V in turn
+  static constexpr int kKeys = DP == 64 ? 128 : 80;  // of a tile
+  static constexpr int kPanels = DP / 64;            // of 64 columns (128 bytes) each
+  static constexpr int kPanel = kKeys * 128;         // bytes
+  static constexpr int kTile = kPanels * kPanel;     // K tile, V tile
+  static constexpr int kQPanel = kRows * 128;
+  static constexpr int kQTile = kPanels * kQPanel;
+  static constexpr int kStages = 6;                  // K and V in turn
   static constexpr int kQOff = 0;
-  static constexpr int kRingOff = 2 * kTile;
-  static constexpr int kOffOff = kRingOff + kStages * kTile;    // int64 row offsets, two tiles
-  static constexpr int kPrepOff = kOffOff + 2 * kKeys * 8;      // per key factors, two tiles
-  static constexpr int kPrepTile = BITS == 16 ? 0 : 5 * kKeys * 4;
+  static constexpr int kRingOff = 2 * kQTile;
+  static constexpr int kPrepOff = kRingOff + kStages * kTile;   // per key factors, two tiles
+  static constexpr int kPrepTile = BITS == 16 ? 0 : (BITS == 8 ? 2 : 4) * kKeys * 4;
   static constexpr int kBarOff = kPrepOff + 2 * kPrepTile;
-  static constexpr int kBars = 2 * kStages + 14;
-  static constexpr int kSmem = kBarOff + kBars * 8 + 64 + 1024;  // + alignment
+  static constexpr int kBars = 2 * kStages + 16;
+  static constexpr int kSmem = kBarOff + kBars * 8 + 128 + 1024;  // + alignment
   static_assert(kSmem <= 227 * 1024, "shared memory");
   using C = std::conditional_t<BITS == 16, T, __half>;
   static constexpr bool kRowFactor = BITS != 16 && std::is_same_v<T, __nv_bfloat16>;
   static constexpr uint32_t kType = std::is_same_v<C, __nv_bfloat16> ? 1u : 0u;
-  // two chains: S (and P) in columns 0 and 128, O in 256 and 256 + DP
+  // columns of tensor memory: S, P and O of chain i
   static constexpr int kCols = 512;
+  static constexpr int kOCol = DP == 64 ? 384 : 256;
+  __device__ static constexpr uint32_t s_at(int i) { return i * 128; }
+  __device__ static constexpr uint32_t p_at(int i) { return DP == 64 ? 256 + i * 64 : i * 128 + 80; }
+  __device__ static constexpr uint32_t o_at(int i) { return kOCol + i * DP; }
+  static_assert(DP == 64 || kKeys + kKeys / 2 <= 128, "S and P of a chain in 128 columns");
 };
 
 // Instruction descriptor: A and B of one 16-bit type, fp32 sums, M = 128; `v`: B is
@@ -90,18 +104,14 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t byt
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Pairs of fp32.
+// Pairs of fp32. (Shared memory is read by its 32-bit address: the compiler does not see
+// through the aligned base and would read generically.)
 struct F2 {
   uint64_t v;
 };
@@ -127,27 +137,45 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   return r;
 }
 
-// The eight K = 16 steps of O += P V, issued from one asm block (their operands are then
-// formed back to back): P 8 columns a step, V 16 keys of 128 bytes.
+// 64 columns x 16 tokens of one page and head (no multicast).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void lds_pairs(uint32_t addr, F2 (&v)[2]) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[0].v), "=l"(v[1].v) : "r"(addr) : "memory");
+}
+
+// Four K = 16 steps of O += P V, issued from one asm block (their operands are then formed
+// back to back): P 8 columns a step, V 16 keys of 128 bytes.
 __device__ __forceinline__ void umma_pv(uint32_t d, uint32_t p, uint64_t v, uint32_t id, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      ".reg .b32 a1, a2, a3, a4, a5, a6, a7;\n\t"
-      ".reg .b64 b1, b2, b3, b4, b5, b6, b7;\n\t"
+      ".reg .b32 a1, a2, a3;\n\t"
+      ".reg .b64 b1, b2, b3;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "setp.eq.u32 q, 0, 0;\n\t"
-      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\tadd.u32 a4, %1, 32;\n\t"
-      "add.u32 a5, %1, 40;\n\tadd.u32 a6, %1, 48;\n\tadd.u32 a7, %1, 56;\n\t"
-      "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\tadd.u64 b4, %2, 512;\n\t"
-      "add.u64 b5, %2, 640;\n\tadd.u64 b6, %2, 768;\n\tadd.u64 b7, %2, 896;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+      "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a4], b4, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a5], b5, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a6], b6, %3, q;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a7], b7, %3, q;\n\t}" ::"r"(d),
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t}" ::"r"(d),
       "r"(p), "l"(v), "r"(id), "r"(accumulate)
       : "memory");
 }
@@ -189,16 +217,18 @@ struct TileArgs {
   int spans;       // key spans of a tile
   int parts;       // 0: rows are written whole; else parts of a row (spans, or 2 spans)
   int tile_rows;   // 256; 128 where both chains take the same rows
+  bool tma;        // the maps of the cache are valid (16 bits, pages of 16 tokens and more)
 };
 
 template <typename T, int BITS, int DP>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, const TileArgs ta) {
+__global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, const TileArgs ta,
+                                                        const __grid_constant__ CUtensorMap map_k,
+                                                        const __grid_constant__ CUtensorMap map_v) {
   using K = Tc<T, BITS, DP>;
   using C = typename K::C;
-  constexpr int kStages = K::kStages;
+  constexpr int kStages = K::kStages, kKeys = K::kKeys;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int64_t* const s_off = reinterpret_cast<int64_t*>(smem + K::kOffOff);
   float* const s_prep = reinterpret_cast<float*>(smem + K::kPrepOff);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + K::kBarOff);
   uint64_t* const full = bars;                  // [stages] rows landed
@@ -208,10 +238,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   uint64_t* const o_done = s_full + 4;          // [2] P V done
   uint64_t* const prep_full = s_full + 6;       // [2]
   uint64_t* const prep_empty = s_full + 8;      // [2]
-  uint64_t* const offs_full = s_full + 10;      // [2] row offsets written
+  uint64_t* const exp_full = s_full + 10;      // [2] exponents of the steps written
   uint64_t* const drain = s_full + 12;          // [2]
+  uint64_t* const s_free = s_full + 14;         // [2] S in registers
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + K::kBars);
   int* const s_odd = reinterpret_cast<int*>(s_tmem + 1);
+  int* const s_exp = s_odd + 1;                 // [2][4] largest step exponent, a loader warp
+  int* const s_e = s_exp + 8;                   // [2] E of the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.kv.head_dim;
   const bool same_rows = ta.tile_rows == kRows;
@@ -272,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     k1 = t0 + static_cast<int>(static_cast<int64_t>(n) * (span + 1) / ta.spans);
   }
   const int n_tiles = k1 - k0;
-  const float cs = fabsf(a.scale) * kLog2e;
+  // (not zero: a score that is masked by -inf stays so times it)
+  const float cs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
 
   // which tiles chain i takes: all, or every second one
   const int step = same_rows ? 2 : 1;
@@ -283,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   if (threadIdx.x == 0) {
     const int chains = chain_b && !same_rows ? 2 : 1;  // that take each tile
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 4);  // one arrival a warp
+      mbar_init(&full[s], 4);  // one arrival a loader warp
       mbar_init(&empty[s], chains);
     }
     for (int i = 0; i < 2; ++i) {
@@ -292,8 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       mbar_init(&o_done[i], 1);
       mbar_init(&prep_full[i], 4);
       mbar_init(&prep_empty[i], 4 * chains);  // softmax warps
-      mbar_init(&offs_full[i], 4);
+      mbar_init(&exp_full[i], 4);
       mbar_init(&drain[i], 1);
+      mbar_init(&s_free[i], 4);
     }
     fence_barrier_init();
     *s_odd = 0;
@@ -334,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       rf = exp2f(static_cast<float>(e));
       inv_factor = 1.f / rf;
     }
-    uint8_t* const dst = smem + K::kQOff + chain * K::kTile + tid * 128;
+    uint8_t* const dst = smem + K::kQOff + chain * K::kQTile + tid * 128;
 #pragma unroll 4
     for (int c = 0; c < D / 8; ++c) {
       uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -364,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           qsum += f.x + f.y;
         }
       }
-      *reinterpret_cast<uint4*>(dst + (c >> 3) * K::kPanel + (((c & 7) ^ (tid & 7)) << 4)) = w;
+      *reinterpret_cast<uint4*>(dst + (c >> 3) * K::kQPanel + (((c & 7) ^ (tid & 7)) << 4)) = w;
     }
     fence_proxy_async_smem();
   }
@@ -381,29 +416,142 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     const int row_bytes = D * BITS / 8;
     constexpr int kChunks = DP * BITS / 128;     // 16-byte pieces of a stored row
     constexpr int kRowsIt = kLoaders / kChunks;  // rows of one step of the loaders
-    constexpr int kIts = kKeys / kRowsIt;
+    constexpr int kIts = (kKeys + kRowsIt - 1) / kRowsIt;
     const int32_t* const table = a.page_table + b * a.page_table_stride;
-    auto page_at = [&](int t) {
-      const int j = (k0 + t) * kKeys + me;
-      return t < n_tiles && j < r.kv_len ? __ldg(table + (j >> a.kv.page_shift)) : -1;
-    };
-    int next_page = page_at(0);
-    // tile t, K then V: stage 2 t + v of the ring
     const int c = me % kChunks, crow = me / kChunks;
-    const bool wide = BITS != 4 || row_bytes % 16 == 0;
-    int done = 0;  // stages whose rows this thread has handed over
-    bool odd = false;
-    auto hand_over = [&]() {  // 16 bits: the oldest stage's copies of this thread have landed
-      const int s = done % kStages;
-      if (done & 1) {
-        // a value tile: look for what is no number where not every row sees every key
-        const int j0 = (k0 + done / 2) * kKeys;
-        if (j0 + kKeys - 1 > tile_min || (a.window > 0 && j0 <= tile_max - a.window)) {
-          if (c * 16 < row_bytes) {
-            for (int it = 0; it < kIts; ++it) {
-              const int row = it * kRowsIt + crow;
-              const uint4 w = *reinterpret_cast<const uint4*>(smem + K::kRingOff + s * K::kTile + (c >> 3) * K::kPanel +
-                                                              row * 128 + (((c & 7) ^ (row & 7)) << 4));
+    const bool mine = c * 16 < row_bytes;
+    const uint32_t ring = smem_u32(smem + K::kRingOff);
+    // This thread's rows of a tile: kIts neighbours from `row0`, so that pages of 16 tokens
+    // and more give it two pages at most. Their ids are asked for a tile ahead.
+    const int row0 = crow * kIts;
+    const int n_rows = mine ? min(kIts, max(0, kKeys - row0)) : 0;
+    const bool two_pages = mask >= 15;
+    int ids[2] = {-1, -1};
+    auto ask_pages = [&](int t) {
+      const int j = (k0 + t) * kKeys + row0, end = min(r.kv_len, j + n_rows);
+      ids[0] = t < n_tiles && j < end ? __ldg(table + (j >> a.kv.page_shift)) : -1;
+      ids[1] = t < n_tiles && j < end ? __ldg(table + ((end - 1) >> a.kv.page_shift)) : -1;
+    };
+    struct Rows {
+      int64_t at[2];  // of the first row, and of the first in its last page
+      int turn;       // rows in the first page
+      int live[2];    // rows below this (from the start, from the turn) have data
+    };
+    auto good_page = [&](int id) {
+      const bool good = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.kv.num_pages);
+      if (!good) set_device_error(kDevBadCachePos);
+      return good;
+    };
+    auto rows_of = [&](int t) {
+      Rows x{{0, 0}, kIts, {0, 0}};
+      const int j = (k0 + t) * kKeys + row0, n = min(r.kv_len - j, n_rows);
+      if (n <= 0) return x;
+      const int off = j & mask;
+      x.turn = min(kIts, mask + 1 - off);
+      if (two_pages) {
+        if (good_page(ids[0])) {
+          x.at[0] = a.kv.row(ids[0], h, off);
+          x.live[0] = min(n, x.turn);
+        }
+        if (n > x.turn && good_page(ids[1])) {
+          x.at[1] = a.kv.row(ids[1], h, 0);
+          x.live[1] = n - x.turn;
+        }
+      }
+      return x;
+    };
+    const int64_t row_step = static_cast<int64_t>(a.kv.token_stride) * 8;
+    // byte offset of row `it` of this thread in tile t, -1 without data
+    auto row_at = [&](const Rows& x, int t, int it) -> int64_t {
+      if (two_pages) {
+        if (it < x.turn) return it < x.live[0] ? x.at[0] + it * row_step : -1;
+        return it - x.turn < x.live[1] ? x.at[1] + (it - x.turn) * row_step : -1;
+      }
+      const int j = (k0 + t) * kKeys + row0 + it;
+      if (it >= n_rows || j >= r.kv_len) return -1;
+      const int id = __ldg(table + (j >> a.kv.page_shift));
+      return good_page(id) ? a.kv.row(id, h, j & mask) : -1;
+    };
+    // 16-byte piece cc of this thread's row `it` in stage g
+    auto place = [&](int g, int cc, int it) {
+      const int row = row0 + it;
+      return ring + g % kStages * K::kTile + (cc >> 3) * K::kPanel + row * 128 + (((cc & 7) ^ (row & 7)) << 4);
+    };
+    // K then V of each tile: stages g = 2 t + v of the ring
+    if constexpr (BITS == 16) {
+      // Tiles that every row sees whole come by TMA, 16 tokens (of one page) and 64 columns
+      // a box, their boxes spread over the loader warps. The others, a few a block, are
+      // copied row by row, which leaves out what lies past the sequence; their values are
+      // then searched for what is no number.
+      const int lw = warp - kLoadWarp;
+      constexpr int kGroups = kKeys / 16;
+      const int panels = (D + 63) / 64;
+      int box_ids[2] = {-1, -1};  // pages of 16-token groups lw and lw + 4 of the next tile
+      auto ask_boxes = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = (k0 + t) * kKeys + (lw + 4 * i) * 16;
+          if (t < n_tiles && lw + 4 * i < kGroups && j < r.kv_len) box_ids[i] = __ldg(table + (j >> a.kv.page_shift));
+        }
+      };
+      ask_boxes(0);
+      bool odd = false;
+      int armed = 0;  // stages filled so far
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        const int j0 = (k0 + t) * kKeys;
+        const bool mixed = j0 + kKeys - 1 > tile_min || (a.window > 0 && j0 <= tile_max - a.window);
+        if (!mixed && ta.tma) {  // (no row sees past the sequence: the tile is inside it)
+          int ids[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ids[i] = box_ids[i];
+            if (lw + 4 * i < kGroups && static_cast<uint32_t>(ids[i]) >= static_cast<uint32_t>(a.kv.num_pages)) {
+              set_device_error(kDevBadCachePos);
+              ids[i] = a.kv.num_pages;  // outside the map: zeros
+            }
+          }
+          ask_boxes(t + 1);
+          const uint32_t bytes = static_cast<uint32_t>(kGroups - lw > 4 ? 2 : 1) * panels * 2048u;
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const int g = 2 * t + v, s = g % kStages;
+            ok = warp_wait(&empty[s], ((g / kStages) & 1) ^ 1u, kDevTimeoutAEmpty);
+            if (!ok) break;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(&full[s], bytes);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int row = (lw + 4 * i) * 16;
+                if (row >= kKeys) break;
+                for (int q = 0; q < panels; ++q)
+                  tma_load_4d(ring + s * K::kTile + q * K::kPanel + row * 128, v ? &map_v : &map_k, &full[s], 64 * q,
+                              (j0 + row) & mask, h, ids[i]);
+              }
+            }
+            __syncwarp();
+            armed = g + 1;
+          }
+          continue;
+        }
+        ask_pages(t);
+        const Rows x = rows_of(t);
+        ask_boxes(t + 1);
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v) {
+          const int g = 2 * t + v, s = g % kStages;
+          ok = warp_wait(&empty[s], ((g / kStages) & 1) ^ 1u, kDevTimeoutAEmpty);
+          if (!ok) break;
+          const uint8_t* const src = (v ? a.kv.v : a.kv.k) + c * 16;
+#pragma unroll 1
+          for (int it = 0; it < n_rows; ++it) {
+            const int64_t ro = row_at(x, t, it);
+            cp16(place(g, c, it), src + max(ro, int64_t{0}), ro < 0 ? 0u : 16u);
+          }
+          cp_commit();
+          cp_wait<0>();
+          if (v == 1 && mixed) {
+            for (int it = 0; it < n_rows; ++it) {
+              const uint4 w = lds128(place(g, c, it));
               const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -412,189 +560,197 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
               }
             }
           }
-        }
-      }
-      fence_proxy_async_smem();
-      warp_arrive(&full[s]);
-      ++done;
-    };
-    for (int t = 0; t < n_tiles && ok; ++t) {
-      // where the tile's rows lie, one a loader
-      const int j = (k0 + t) * kKeys + me;
-      int64_t off = -1, soff = 0;
-      if (j < r.kv_len) {
-        const int page = next_page;
-        if (page >= 0 && page < a.kv.num_pages) {
-          off = a.kv.row(page, h, j & mask);
-          if constexpr (BITS != 16) soff = a.kv.scale_row(page, h, j & mask);
-        } else {
-          set_device_error(kDevBadCachePos);
-        }
-      }
-      next_page = page_at(t + 1);
-      int64_t* const offs = s_off + (t & 1) * kKeys;
-      offs[me] = off;
-      float2 ksc = make_float2(0.f, 0.f), vsc = ksc;
-      if constexpr (BITS != 16) {
-        if (off >= 0) {
-          if constexpr (BITS == 8) {
-            ksc.x = __ldg(a.kv.k_scale + soff);
-            vsc.x = __ldg(a.kv.v_scale + soff);
-          } else {
-            ksc = __ldg(reinterpret_cast<const float2*>(a.kv.k_scale + soff));
-            vsc = __ldg(reinterpret_cast<const float2*>(a.kv.v_scale + soff));
-          }
-        }
-      }
-      warp_arrive(&offs_full[t & 1]);
-      ok = warp_wait(&offs_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
-#pragma unroll 1
-      for (int v = 0; v < 2 && ok; ++v) {
-        const int g = 2 * t + v, s = g % kStages;
-        const uint8_t* const src = v ? a.kv.v : a.kv.k;
-        uint8_t* const dst = smem + K::kRingOff + s * K::kTile;
-        uint4 raw[BITS == 16 ? 1 : kIts];
-        if constexpr (BITS != 16) {
-          // codes first: their way from memory overlaps the wait
-#pragma unroll
-          for (int it = 0; it < kIts; ++it) {
-            const int64_t ro = offs[it * kRowsIt + crow];
-            raw[it] = make_uint4(0u, 0u, 0u, 0u);
-            if (ro >= 0 && c * 16 < row_bytes) {
-              if (wide) {
-                raw[it] = __ldg(reinterpret_cast<const uint4*>(src + ro + c * 16));
-              } else {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + ro + c * 16));
-                raw[it].x = x.x;
-                raw[it].y = x.y;
-                if (c * 16 + 8 < row_bytes) {
-                  const uint2 y = __ldg(reinterpret_cast<const uint2*>(src + ro + c * 16 + 8));
-                  raw[it].z = y.x;
-                  raw[it].w = y.y;
-                }
-              }
-            }
-          }
-        }
-        if (!__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&empty[s]), ((g / kStages) & 1) ^ 1u))) {
-          if constexpr (BITS == 16) {
-            // nothing to issue: hand over what is on its way
-            if (done < g) {
-              cp_wait<0>();
-              hand_over();
-            }
-          }
-          ok = warp_wait(&empty[s], ((g / kStages) & 1) ^ 1u, kDevTimeoutAEmpty);
-          if (!ok) break;
-        }
-        if constexpr (BITS == 16) {
-          if (c * 16 < row_bytes) {
-#pragma unroll
-            for (int it = 0; it < kIts; ++it) {
-              const int row = it * kRowsIt + crow;
-              const int64_t ro = offs[row];
-              cp16(smem_u32(dst + (c >> 3) * K::kPanel + row * 128 + (((c & 7) ^ (row & 7)) << 4)),
-                   src + (ro < 0 ? 0 : ro + c * 16), ro < 0 ? 0u : 16u);
-            }
-          }
-          cp_commit();
-          if (done < g) {
-            cp_wait<1>();
-            hand_over();
-          }
-        } else {
-          if (v == 0) {
-            // the key's factors: a = s c, log2 t, 1 / t, z c, y / t, with c = scale log2(e)
-            ok = warp_wait(&prep_empty[t & 1], ((t >> 1) & 1) ^ 1u, kDevTimeoutAEmpty);
-            if (!ok) break;
-            float* const prep = s_prep + (t & 1) * 5 * kKeys;
-            const float vstep = vsc.x < kMinScale ? kMinScale : vsc.x;  // a step of zero; a NaN stays
-            const float lv = lg2(vstep), inv = ex2(-lv);
-            prep[me] = ksc.x * cs;
-            prep[kKeys + me] = lv;
-            // a row that sees a poisoned key has a NaN weight; one that does not has weight
-            // zero, which must meet a number here
-            prep[2 * kKeys + me] = inv < INFINITY ? inv : 0.f;
-            if constexpr (BITS == 4) {
-              const float zr = fmaf(8.f, vsc.x, vsc.y) / vstep;
-              prep[3 * kKeys + me] = fmaf(8.f, ksc.x, ksc.y) * cs;
-              prep[4 * kKeys + me] = fabsf(zr) < INFINITY ? zr : 0.f;
-            }
-            warp_arrive(&prep_full[t & 1]);
-          }
-          if (c * 16 < row_bytes) {
-#pragma unroll
-            for (int it = 0; it < kIts; ++it) {
-              const int row = it * kRowsIt + crow;
-              const uint32_t ws[4] = {raw[it].x, raw[it].y, raw[it].z, raw[it].w};
-              constexpr int kOut = 16 / BITS;  // 16-byte pieces that a piece of codes becomes
-#pragma unroll
-              for (int o = 0; o < kOut; ++o) {
-                uint4 w;
-                if constexpr (BITS == 8) {
-                  uint32_t x[2], y[2];
-                  unpack8(ws[2 * o], x);
-                  unpack8(ws[2 * o + 1], y);
-                  w = make_uint4(x[0], x[1], y[0], y[1]);
-                } else {
-                  uint32_t x[4];
-                  unpack4(ws[o], x);
-                  w = make_uint4(x[0], x[1], x[2], x[3]);
-                }
-                const int cc = c * kOut + o;
-                *reinterpret_cast<uint4*>(dst + (cc >> 3) * K::kPanel + row * 128 + (((cc & 7) ^ (row & 7)) << 4)) = w;
-              }
-            }
-          }
           fence_proxy_async_smem();
           warp_arrive(&full[s]);
+          armed = g + 1;
         }
       }
-    }
-    if constexpr (BITS == 16) {
-      cp_wait<0>();
-      if (ok && done < 2 * n_tiles) hand_over();
       if (odd) *s_odd = 1;
+      // copies by TMA that no product has waited for (a wait ran out) must land before the
+      // block leaves its shared memory
+      if (!ok) {
+        for (int s = 0; s < kStages && s < armed; ++s) mbar_wait_drain(&full[s], ((armed - 1 - s) / kStages) & 1);
+      }
+    } else {
+      const bool wide = BITS == 8 || row_bytes % 16 == 0;
+      int exp_now = -126;  // E
+      // Steps of the tile's keys, one a loader, two tiles ahead: of the tile after the one
+      // whose codes are being asked for the loaders exchange the largest exponent.
+      float2 ksc = make_float2(0.f, 0.f), vsc = ksc;
+      auto ask_steps = [&](int t) {
+        ksc = vsc = make_float2(0.f, 0.f);
+        const int j = (k0 + t) * kKeys + me;
+        if (me >= kKeys || t >= n_tiles || j >= r.kv_len) return;
+        const int page = __ldg(table + (j >> a.kv.page_shift));
+        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.kv.num_pages)) return;
+        const int64_t at = a.kv.scale_row(page, h, j & mask);
+        if constexpr (BITS == 8) {
+          ksc.x = __ldg(a.kv.k_scale + at);
+          vsc.x = __ldg(a.kv.v_scale + at);
+        } else {
+          ksc = __ldg(reinterpret_cast<const float2*>(a.kv.k_scale + at));
+          vsc = __ldg(reinterpret_cast<const float2*>(a.kv.v_scale + at));
+        }
+      };
+      auto tell_exponent = [&](int t) {
+        const int e = __reduce_max_sync(0xffffffffu, vsc.x < INFINITY ? ilogbf(fmaxf(vsc.x, kMinScale)) : -126);
+        if (lane == 0) s_exp[(t & 1) * 4 + (me >> 5)] = e;
+        warp_arrive(&exp_full[t & 1]);
+      };
+      auto fetch_codes = [&](const Rows& x, int t, const uint8_t* base, uint4 (&raw)[kIts]) {
+        if (x.live[0] == kIts && wide) {  // all in one page, as nearly always
+          const uint8_t* src = base + x.at[0] + c * 16;
+#pragma unroll
+          for (int it = 0; it < kIts; ++it, src += row_step) raw[it] = __ldg(reinterpret_cast<const uint4*>(src));
+          return;
+        }
+#pragma unroll
+        for (int it = 0; it < kIts; ++it) {
+          raw[it] = make_uint4(0u, 0u, 0u, 0u);
+          const int64_t ro = row_at(x, t, it);
+          if (ro < 0) continue;
+          const uint8_t* const src = base + ro + c * 16;
+          if (wide) {
+            raw[it] = __ldg(reinterpret_cast<const uint4*>(src));
+          } else {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src));
+            raw[it].x = x.x;
+            raw[it].y = x.y;
+            if (c * 16 + 8 < row_bytes) {
+              const uint2 y = __ldg(reinterpret_cast<const uint2*>(src + 8));
+              raw[it].z = y.x;
+              raw[it].w = y.y;
+            }
+          }
+        }
+      };
+      auto store_codes = [&](int g, const uint4 (&raw)[kIts]) {
+        ok = warp_wait(&empty[g % kStages], ((g / kStages) & 1) ^ 1u, kDevTimeoutAEmpty);
+        if (!ok) return;
+        {
+#pragma unroll
+          for (int it = 0; it < kIts; ++it) {
+            if (it >= n_rows) break;
+            const uint32_t ws[4] = {raw[it].x, raw[it].y, raw[it].z, raw[it].w};
+            constexpr int kOut = 16 / BITS;  // 16-byte pieces that a piece of codes becomes
+#pragma unroll
+            for (int o = 0; o < kOut; ++o) {
+              uint4 w;
+              if constexpr (BITS == 8) {
+                uint32_t x[2], y[2];
+                unpack8(ws[2 * o], x);
+                unpack8(ws[2 * o + 1], y);
+                w = make_uint4(x[0], x[1], y[0], y[1]);
+              } else {
+                uint32_t x[4];
+                unpack4(ws[o], x);
+                w = make_uint4(x[0], x[1], x[2], x[3]);
+              }
+              sts128(place(g, c * kOut + o, it), w);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&full[g % kStages]);
+      };
+      auto factors = [&](int t, float2 kstep, float2 vstep) {
+        ok = warp_wait(&prep_empty[t & 1], ((t >> 1) & 1) ^ 1u, kDevTimeoutAEmpty) &&
+             warp_wait(&exp_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
+        if (!ok) return;
+        // the key's factors: a = s c, t / 2^E (and z c, y / t), with c = scale log2(e). A
+        // poisoned step of either makes a NaN in a, which reaches the weights of the rows
+        // that see the key and no others; the rest must then be numbers.
+#pragma unroll
+        for (int w = 0; w < 4; ++w) exp_now = max(exp_now, s_exp[(t & 1) * 4 + w]);
+        if (me < kKeys) {
+          float* const prep = s_prep + (t & 1) * (K::kPrepTile / 4);
+          const float vs = vstep.x < kMinScale ? kMinScale : vstep.x;  // a step of zero; a NaN stays
+          bool bad = !(vs < INFINITY);
+          if constexpr (BITS == 4) {
+            const float zr = fmaf(8.f, vstep.x, vstep.y) / vs;
+            bad = bad || !(fabsf(zr) < INFINITY);
+            prep[2 * kKeys + me] = fmaf(8.f, kstep.x, kstep.y) * cs;
+            prep[3 * kKeys + me] = bad ? 0.f : zr;
+          }
+          prep[me] = bad ? NAN : kstep.x * cs;
+          prep[kKeys + me] = bad ? 0.f : vs * exp2f(static_cast<float>(-exp_now));
+          if (me == 0) s_e[t & 1] = exp_now;
+        }
+        warp_arrive(&prep_full[t & 1]);
+      };
+      // each stage's codes are asked for a stage ahead
+      uint4 raw_k[kIts], raw_v[kIts];
+      ask_steps(0);
+      ask_pages(0);
+      Rows x = rows_of(0);
+      ask_pages(1);
+      if (n_tiles > 0) {
+        fetch_codes(x, 0, a.kv.k, raw_k);
+        tell_exponent(0);
+      }
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        fetch_codes(x, t, a.kv.v, raw_v);
+        const float2 kstep = ksc, vstep = vsc;
+        ask_steps(t + 1);
+        factors(t, kstep, vstep);
+        if (ok) store_codes(2 * t, raw_k);
+        if (!ok) break;
+        if (t + 1 < n_tiles) {
+          x = rows_of(t + 1);
+          ask_pages(t + 2);
+          fetch_codes(x, t + 1, a.kv.k, raw_k);
+          tell_exponent(t + 1);
+        }
+        store_codes(2 * t + 1, raw_v);
+      }
     }
   } else if (warp >= kMmaWarp) {
     // ---------------------------------------------------------- products of one chain
     regs_down<kOtherRegs>();
     const int i = warp - kMmaWarp;
     if (i == 0 || (i == 1 && chain_b)) {
-      const uint32_t s_col = tmem + i * 128, o_col = tmem + 256 + i * DP;
+      const uint32_t s_col = tmem + K::s_at(i), p_col = tmem + K::p_at(i), o_col = tmem + K::o_at(i);
       const uint32_t id_s = idesc(K::kType, kKeys, false), id_o = idesc(K::kType, D, true);
-      const uint32_t q_addr = smem_u32(smem + K::kQOff + i * K::kTile);
+      const uint32_t q_addr = smem_u32(smem + K::kQOff + i * K::kQTile);
       const int ks = D / 16;
-      int n = 0;  // tiles of this chain so far
-      for (int t = chain_first(i); t < n_tiles && ok; t += step, ++n) {
-        const int gk = 2 * t, gv = gk + 1;
-        ok = warp_wait(&full[gk % kStages], (gk / kStages) & 1, kDevTimeoutAFull);
-        // S overwrites P: the last product with it must have ended
-        if (ok && n > 0) ok = warp_wait(&o_done[i], (n - 1) & 1, kDevTimeoutAccFull);
-        if (!ok) break;
+      // S of tile t, once its keys are there
+      auto product_s = [&](int t) {
+        const int g = 2 * t, s = g % kStages;
+        ok = warp_wait(&full[s], (g / kStages) & 1, kDevTimeoutAFull);
+        if (!ok) return;
         tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + K::kRingOff + (gk % kStages) * K::kTile);
         if (elect_one()) {
+          const uint32_t k_addr = smem_u32(smem + K::kRingOff + s * K::kTile);
           int k = 0;
           for (; k + 4 <= ks; k += 4)
-            umma_f16_k64(s_col, sdesc_sw128(q_addr + (k >> 2) * K::kPanel), sdesc_sw128(k_addr + (k >> 2) * K::kPanel), id_s, k > 0);
-          for (; k < ks; ++k) {
-            const uint32_t at = (k >> 2) * K::kPanel + (k & 3) * 32;
-            umma_f16(s_col, sdesc_sw128(q_addr + at), sdesc_sw128(k_addr + at), id_s, k > 0);
-          }
+            umma_f16_k64(s_col, sdesc_sw128(q_addr + (k >> 2) * K::kQPanel), sdesc_sw128(k_addr + (k >> 2) * K::kPanel), id_s, k > 0);
+          for (; k < ks; ++k)
+            umma_f16(s_col, sdesc_sw128(q_addr + (k >> 2) * K::kQPanel + (k & 3) * 32),
+                     sdesc_sw128(k_addr + (k >> 2) * K::kPanel + (k & 3) * 32), id_s, k > 0);
           umma_commit(&s_full[i]);
-          umma_commit(&empty[gk % kStages]);
+          umma_commit(&empty[s]);
         }
         __syncwarp();
-        ok = warp_wait(&full[gv % kStages], (gv / kStages) & 1, kDevTimeoutAFull) &&
-             warp_wait(&p_full[i], n & 1, kDevTimeoutAccEmpty);
+      };
+      int t = chain_first(i);
+      if (t < n_tiles) product_s(t);
+      for (int n = 0; t < n_tiles && ok; t += step, ++n) {
+        if (t + step < n_tiles) {
+          // the next tile's S, once this one's is in registers: under the exponentials
+          ok = warp_wait(&s_free[i], n & 1, kDevTimeoutAccEmpty);
+          if (ok) product_s(t + step);
+        }
+        const int g = 2 * t + 1, s = g % kStages;
+        ok = ok && warp_wait(&full[s], (g / kStages) & 1, kDevTimeoutAFull) && warp_wait(&p_full[i], n & 1, kDevTimeoutAccEmpty);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t v_addr = smem_u32(smem + K::kRingOff + (gv % kStages) * K::kTile);
         if (elect_one()) {
-          umma_pv(o_col, s_col, sdesc_v(v_addr, K::kPanel), id_o, n > 0);
+          const uint64_t v = sdesc_v(smem_u32(smem + K::kRingOff + s * K::kTile), K::kPanel);
+          umma_pv(o_col, p_col, v, id_o, n > 0);
+          if constexpr (kKeys == 128) umma_pv(o_col, p_col + 32, v + 512, id_o, 1);
+          else umma_f16_ts(o_col, p_col + 32, v + 512, id_o, 1);
           umma_commit(&o_done[i]);
-          umma_commit(&empty[gv % kStages]);
+          umma_commit(&empty[s]);
         }
         __syncwarp();
       }
@@ -607,17 +763,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     if (chain == 0 || chain_b) {
     // ---------------------------------------------------------- softmax: a thread a row
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp
-    const uint32_t s_col = tmem + lanes + chain * 128, o_col = tmem + lanes + 256 + chain * DP;
+    const uint32_t s_col = tmem + lanes + K::s_at(chain), p_col = tmem + lanes + K::p_at(chain),
+                   o_col = tmem + lanes + K::o_at(chain);
     // positions of this warp's first and last row
     const int w_row = my_row - lane;
     const int w_min = pos0 + (row0 + w_row) / a.group;
     const int w_max = pos0 + (row0 + min(w_row + 31, max(rows, 1) - 1)) / a.group;
     float ref = -INFINITY, l = 0.f, zacc = 0.f;
+    int e_now = -126;  // E of the sums so far
     int n = 0;
     for (int t = chain_first(chain); t < n_tiles && ok; t += step, ++n) {
       const int j0 = (k0 + t) * kKeys;
       const bool whole = j0 + kKeys - 1 <= w_min && (a.window <= 0 || j0 > w_max - a.window);
-      const float* const prep = s_prep + (t & 1) * 5 * kKeys;
+      const uint32_t prep = smem_u32(s_prep + (t & 1) * (K::kPrepTile / 4));
       if constexpr (BITS != 16) ok = warp_wait(&prep_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
       ok = ok && warp_wait(&s_full[chain], n & 1, kDevTimeoutAccFull);
       if (!ok) break;
@@ -625,24 +783,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       uint32_t s[kKeys];
 #pragma unroll
       for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(s_col + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
+      if constexpr (kKeys % 32 != 0) tmem_ld16(s_col + kKeys - 16, reinterpret_cast<uint32_t(&)[16]>(s[kKeys - 16]));
       tmem_ld_wait();
+      tc_fence_before();
+      warp_arrive(&s_free[chain]);
       auto sf = [&](int j) { return __uint_as_float(s[j]); };
       if constexpr (BITS != 16) {
-        // scores of codes, with the values' steps in them
+        // scores of codes
         const F2 qs2 = f2(qsum, qsum), rf2 = f2(rf, rf);
 #pragma unroll
         for (int j = 0; j < kKeys; j += 4) {
-          const float4 aj = *reinterpret_cast<const float4*>(prep + j);
-          const float4 lv = *reinterpret_cast<const float4*>(prep + kKeys + j);
-          float4 zj = make_float4(0.f, 0.f, 0.f, 0.f);
-          if constexpr (BITS == 4) zj = *reinterpret_cast<const float4*>(prep + 3 * kKeys + j);
+          F2 a2[2], z2[2];
+          lds_pairs(prep + 4 * j, a2);
+          if constexpr (BITS == 4) lds_pairs(prep + 4 * (2 * kKeys + j), z2);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const F2 a2 = e ? f2(aj.z, aj.w) : f2(aj.x, aj.y), l2 = e ? f2(lv.z, lv.w) : f2(lv.x, lv.y);
-            const F2 z2 = e ? f2(zj.z, zj.w) : f2(zj.x, zj.y), s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
+            const F2 s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
             F2 x;
-            if constexpr (K::kRowFactor) x = fma2(BITS == 4 ? fma2(s2, a2, mul2(qs2, z2)) : mul2(s2, a2), rf2, l2);
-            else x = fma2(s2, a2, BITS == 4 ? fma2(qs2, z2, l2) : l2);
+            if constexpr (BITS == 4) x = fma2(s2, a2[e], mul2(qs2, z2[e]));
+            else x = mul2(s2, a2[e]);
+            if constexpr (K::kRowFactor) x = mul2(x, rf2);
             float x0, x1;
             split(x, x0, x1);
             s[j + 2 * e] = __float_as_uint(x0);
@@ -664,12 +824,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * (BITS == 16 ? cs : 1.f);
       // a row whose reference is not set yet, or is left behind, takes its maximum
       const bool behind = ref == -INFINITY ? top > -INFINITY : top > ref + kSlack;
-      if (__any_sync(0xffffffffu, behind)) {
+      int e_tile = e_now;
+      if constexpr (BITS != 16) e_tile = s_e[t & 1];
+      if (__any_sync(0xffffffffu, behind || e_tile != e_now)) {
         const float now = behind ? top : ref;
-        const float keep = now == -INFINITY ? 1.f : ex2(ref - now);  // ref = -inf: 0
+        float keep = now == -INFINITY ? 1.f : ex2(ref - now);  // ref = -inf: 0
         l *= keep;
-        zacc *= keep;
         ref = now;
+        if constexpr (BITS != 16) {
+          keep *= ex2(static_cast<float>(max(e_now - e_tile, -126)));
+          zacc *= keep;
+          e_now = e_tile;
+        }
         if (n > 0) {
           ok = warp_wait(&o_done[chain], (n - 1) & 1, kDevTimeoutAccFull);
           if (!ok) break;
@@ -688,37 +854,47 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const float base = ref == -INFINITY ? 0.f : ref;
       const F2 base2 = f2(-base, -base), cs2 = f2(cs, cs);
       F2 lt[2] = {f2(l, 0.f), f2(0.f, 0.f)}, zt = f2(zacc, 0.f);
+      uint32_t p[kKeys / 2];
+      auto weights = [&](int from_i, int to_i) {  // pairs of keys
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const int j = 64 * half + 2 * i;
-          float4 iv, zr;
-          if constexpr (BITS != 16) iv = *reinterpret_cast<const float4*>(prep + 2 * kKeys + j);
-          if constexpr (BITS == 4) zr = *reinterpret_cast<const float4*>(prep + 4 * kKeys + j);
+        for (int i = from_i; i < to_i; i += 2) {
+          const int j = 2 * i;
+          F2 tv[2], zr[2];
+          if constexpr (BITS != 16) lds_pairs(prep + 4 * (kKeys + j), tv);
+          if constexpr (BITS == 4) lds_pairs(prep + 4 * (3 * kKeys + j), zr);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const F2 s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
             float y0, y1;
             split(BITS == 16 ? fma2(s2, cs2, base2) : add2(s2, base2), y0, y1);
-            const float w0 = ex2(y0), w1 = ex2(y1);
+            F2 w = f2(ex2(y0), ex2(y1));
+            lt[e] = add2(lt[e], w);
+            if constexpr (BITS != 16) w = mul2(w, tv[e]);
+            float w0, w1;
+            split(w, w0, w1);
             p[i + e] = pack2<C>(w0, w1);
-            if constexpr (BITS == 16) {
-              lt[e] = add2(lt[e], f2(w0, w1));
-            } else {
-              lt[e] = fma2(f2(w0, w1), e ? f2(iv.z, iv.w) : f2(iv.x, iv.y), lt[e]);
-              if constexpr (BITS == 4) {
-                // the rounded weights, so that their rounding scales with the value and
-                // not with the code's distance from 8
-                const float2 f = unpack2<C>(p[i + e]);
-                zt = fma2(f2(f.x, f.y), e ? f2(zr.z, zr.w) : f2(zr.x, zr.y), zt);
-              }
+            if constexpr (BITS == 4) {
+              // the rounded weights, so that their rounding scales with the value and not
+              // with the code's distance from 8 (but below fp16's normal range, where a
+              // row of equal values comes with its tiny step, the weight itself)
+              const float2 f = unpack2<C>(p[i + e]);
+              zt = fma2(f2(w0 < kHalfMin ? w0 : f.x, w1 < kHalfMin ? w1 : f.y), zr[e], zt);
             }
           }
         }
-        tmem_st32(s_col + 32 * half, p);
+      };
+      // (asked now, so that the answer is there when P goes out)
+      const bool p_free = n == 0 || mbar_test_wait(smem_u32(&o_done[chain]), (n - 1) & 1);
+      weights(0, 32);
+      if (!__all_sync(0xffffffffu, p_free)) {
+        ok = warp_wait(&o_done[chain], (n - 1) & 1, kDevTimeoutAccFull);
+        if (!ok) break;
       }
+      tc_fence_after();
+      tmem_st32(p_col, reinterpret_cast<uint32_t(&)[32]>(p[0]));
+      weights(32, kKeys / 2);
+      if constexpr (kKeys == 128) tmem_st32(p_col + 32, reinterpret_cast<uint32_t(&)[32]>(p[32]));
+      else tmem_st8(p_col + 32, reinterpret_cast<uint32_t(&)[8]>(p[32]));
       {
         float x0, x1, y0, y1;
         split(lt[0], x0, x1);
@@ -739,6 +915,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const bool in = my_row < rows;
       const int tok = (row0 + my_row) / a.group, hh = (row0 + my_row) % a.group;
       const int64_t at = static_cast<int64_t>(r.start + tok) * a.q_heads + h * a.group + hh;
+      const float up = BITS == 16 ? 1.f : exp2f(static_cast<float>(e_now));  // 2^E
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       const int part = same_rows ? 2 * span + chain : span;
       const int64_t slot = ((static_cast<int64_t>(tile) * a.kv.kv_heads + h) * max(ta.parts, 1) + part) * ta.tile_rows + my_row;
@@ -755,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           for (int e = 0; e < 16; ++e) {
             // a 4-bit row's columns stand in the order its codes unpack
             const int d = BITS == 4 ? (e & 8) + place4(e & 7) : e;
-            x[d] = __uint_as_float(o[e]) + zacc;
+            x[d] = BITS == 16 ? __uint_as_float(o[e]) : (__uint_as_float(o[e]) + zacc) * up;
           }
         } else {
 #pragma unroll
@@ -852,13 +1029,40 @@ Plan plan(const AttnArgs& a, int max_q_len, int max_kv_len) {
   p.tile_rows = static_cast<int64_t>(max_q_len) * a.group <= kRows ? kRows : 2 * kRows;
   p.tiles = std::min<int64_t>(rows, rows / p.tile_rows + a.num_seqs);  // a partial one each
   const int64_t blocks = p.tiles * a.kv.kv_heads;
-  // spans until the blocks fill the machine, none shorter than four tiles of keys
-  const int64_t most = std::max<int64_t>(1, max_kv_len / (4 * kKeys));
+  // spans until the blocks fill the machine, none shorter than 512 keys
+  const int64_t most = std::max<int64_t>(1, max_kv_len / 512);
   p.spans = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(device_sm_count() / std::max<int64_t>(1, blocks), most)));
   p.parts = p.tile_rows == kRows ? 2 * p.spans : p.spans > 1 ? p.spans : 0;
   return p;
 }
 size_t round256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+  }();
+  return fn;
+}
+
+// Keys or values of a 16-bit cache as [page][head][token][column], 16 tokens x 64 columns
+// a box. False where the map cannot be made; the rows are then copied one by one.
+bool cache_map(CUtensorMap* m, const KvDev& kv, const void* base, bool bf16) {
+  const auto fn = encode_fn();
+  if (fn == nullptr || kv.page_shift < 4) return false;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.head_dim), cuuint64_t{1} << kv.page_shift,
+                        static_cast<cuuint64_t>(kv.kv_heads), static_cast<cuuint64_t>(kv.num_pages)};
+  cuuint64_t strides[3] = {cuuint64_t{kv.token_stride} * 8, cuuint64_t{kv.head_stride} * 8, cuuint64_t{kv.page_stride} * 8};
+  cuuint32_t box[4] = {64, 16, 1, 1};
+  cuuint32_t ones[4] = {1, 1, 1, 1};
+  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+            strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 template <typename T, int BITS, int DP>
 struct Many {
@@ -880,7 +1084,11 @@ struct Many {
     ta.spans = p.spans;
     ta.parts = p.parts;
     ta.tile_rows = p.tile_rows;
-    e = launch_dep(k_attn_many<T, BITS, DP>, dim3(static_cast<unsigned>(heads * p.spans)), dim3(kThreads), K::kSmem, s, a, ta);
+    CUtensorMap maps[2] = {};
+    ta.tma = BITS == 16 && cache_map(&maps[0], a.kv, a.kv.k, std::is_same_v<T, __nv_bfloat16>) &&
+             cache_map(&maps[1], a.kv, a.kv.v, std::is_same_v<T, __nv_bfloat16>);
+    e = launch_dep(k_attn_many<T, BITS, DP>, dim3(static_cast<unsigned>(heads * p.spans)), dim3(kThreads), K::kSmem, s, a, ta,
+                   maps[0], maps[1]);
     if (e != cudaSuccess || (BITS != 16 && p.parts == 0)) return e;
     return launch_dep(k_attn_tiles<T, BITS, DP>, dim3(static_cast<unsigned>(heads), p.parts > 0 ? 32u : 1u), dim3(kJoinThreads), 0,
                       s, a, ta);

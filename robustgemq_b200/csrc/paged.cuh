@@ -87,6 +87,7 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
 }
 
+constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14, the smallest normal fp16 number
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

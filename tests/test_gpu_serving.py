@@ -167,6 +167,39 @@ def test_attention_sharp_and_flat_scores(gain, q_len):
     Batch([(q_len, 1500)], 4, 1, 128, 32, 8, B16, q_gain=gain).check()
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n,length", [(1, 300), (9, 700), (200, 600)])
+def test_attention_steps_of_every_size(bits, n, length):
+    """Rows of equal values (a step of 2^-64, all of the value in the base), zero rows, and
+    steps that differ by 2^20 between positions, larger ones later."""
+    b = Batch([(n, length)], 4, 2, 64, 16, bits, H16, seed=n)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    k = torch.randn((length, 2, 64), generator=g, device="cuda").half()
+    v = torch.randn((length, 2, 64), generator=g, device="cuda").half()
+    v[::3] = torch.randn((v[::3].shape[0], 2, 1), generator=g, device="cuda").half()
+    v[1::7] = 0.0
+    k[5::9] = 0.0
+    k[7::11] = 0.25
+    v[length // 2:] *= 2.0 ** 10
+    v[:length // 4] *= 2.0 ** -10
+    b.put(0, torch.arange(length, device="cuda"), k, v)
+    b.k[0] = torch.from_numpy(stored_values(k.float().cpu().numpy(), bits)).cuda()
+    b.v[0] = torch.from_numpy(stored_values(v.float().cpu().numpy(), bits)).cuda()
+    b.check()
+    # nothing but rows of equal values
+    v = torch.randn((length, 2, 1), generator=g, device="cuda").half().expand(length, 2, 64).contiguous()
+    b.put(0, torch.arange(length, device="cuda"), k, v)
+    b.v[0] = torch.from_numpy(stored_values(v.float().cpu().numpy(), bits)).cuda()
+    b.check()
+
+
+@pytest.mark.parametrize("n", [1, 40, 150])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_attention_negative_scale(n, bits):
+    Batch([(n, 400)], 4, 2, 64, 16, bits, B16).check(scale=-0.2)
+    Batch([(n, 400)], 4, 2, 64, 16, bits, H16).check(scale=0.0)
+
+
 @pytest.mark.parametrize("bits", [16, 8, 4])
 @pytest.mark.parametrize("n,length,hit", [(1, 300, 100), (6, 300, 297), (6, 300, 100), (200, 500, 400), (200, 500, 350)])
 @pytest.mark.parametrize("which", ["k", "v", "both"])
