@@ -27,9 +27,9 @@
 // 2^8 (in 16 bits 2^8 is as exact as 1), so that the sums in tensor memory are rarely
 // touched between products.
 //
-// Where few tiles there are to fill the machine, each takes part of the keys and
-// k_attn_tiles adds the parts up; with at most 128 rows a KV head both chains take the
-// same rows and every second tile of keys each.
+// Row tiles that do not fill a last round of the machine (all of them, where they are few)
+// are cut along their keys until they do, and k_attn_tiles adds the parts up; with at most
+// 128 rows a KV head both chains take the same rows and every second tile of keys each.
 #define GEMQ_OWN_ERROR_WORDS  // compiled without relocatable device code, for setmaxnreg
 #include <cudaTypedefs.h>
 
@@ -205,19 +205,41 @@ __device__ __forceinline__ void unpack4(uint32_t w, uint32_t (&o)[4]) {  // eigh
 // Which element of its eight stands at place p of a 4-bit row's columns.
 __host__ __device__ constexpr int place4(int p) { return (p >> 1) + 4 * (p & 1); }
 
+// What a block did, for k_attn_tiles.
 struct TileNote {
   int start, row0, rows, head, seq;
   int odd;  // a value that is no number lay in a tile that not every row sees whole
 };
+// How the items (row tiles x KV heads) fall to the blocks: the first `whole` to one each,
+// the rest to `spans` each.
+struct Shares {
+  int items, whole, spans;
+};
 
 struct TileArgs {
-  TileNote* note;  // [tiles][kv_heads][spans]
-  float* o;        // [tiles][kv_heads][parts][tile rows][DP], with parts only
-  float2* ml;      // [tiles][kv_heads][parts][tile rows]
-  int spans;       // key spans of a tile
-  int parts;       // 0: rows are written whole; else parts of a row (spans, or 2 spans)
+  TileNote* note;  // [blocks]
+  Shares* shares;
+  float* o;        // [slots][tile rows][DP]: parts of rows
+  float2* ml;      // [slots][tile rows]
+  int sms;
+  int most_spans;  // of an item
   int tile_rows;   // 256; 128 where both chains take the same rows
   bool tma;        // the maps of the cache are valid (16 bits, pages of 16 tokens and more)
+
+  __device__ __forceinline__ Shares share(int items) const {
+    Shares s;
+    s.items = items;
+    s.whole = items / sms * sms;
+    s.spans = items > s.whole ? min(most_spans, max(1, sms / (items - s.whole))) : 1;
+    return s;
+  }
+  // the first slot of block i's parts (one, or a chain each)
+  __device__ __forceinline__ int slot(const Shares& s, int i) const {
+    return tile_rows == kRows ? 2 * i : i - s.whole;
+  }
+  __device__ __forceinline__ bool cut(const Shares& s, int i) const {
+    return tile_rows == kRows || (i >= s.whole && s.spans > 1);
+  }
 };
 
 template <typename T, int BITS, int DP>
@@ -258,16 +280,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   // ------------------------------------------------------------ this block's rows and keys
   // Tiles in descending order of their position: of a causal sequence's tiles the last
   // ones are the longest, and the short ones fill the machine's end.
-  const int span = static_cast<int>(blockIdx.x) % ta.spans;
-  const int h = static_cast<int>(blockIdx.x) / ta.spans % a.kv.kv_heads;
-  const int tile_back = static_cast<int>(blockIdx.x) / ta.spans / a.kv.kv_heads;
   auto tiles_of = [&](int b) { return (seq_range(a, b).q_len * a.group + ta.tile_rows - 1) / ta.tile_rows; };
   int total = 0;
   for (int b = lane; b < a.num_seqs; b += 32) total += tiles_of(b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const int tile = total - 1 - tile_back;
-  bool work = tile >= 0;
+  const int block = static_cast<int>(blockIdx.x);
+  const Shares shares = ta.share(total * a.kv.kv_heads);
+  if (block == 0 && threadIdx.x == 0) *ta.shares = shares;
+  const bool own_item = block < shares.whole;
+  const int spans = own_item ? 1 : shares.spans;
+  const int span = own_item ? 0 : (block - shares.whole) % spans;
+  const int item = own_item ? block : shares.whole + (block - shares.whole) / spans;
+  const int h = item % a.kv.kv_heads;
+  const int tile = total - 1 - item / a.kv.kv_heads;
+  const bool work = item < shares.items;
   int b = 0, first_tile = 0;
   if (work) {
     int base = 0;
@@ -301,8 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   if (work) {
     const int lo = a.window > 0 ? max(0, tile_min - a.window + 1) : 0;
     const int t0 = lo / kKeys, n = max(0, (tile_max + 1 + kKeys - 1) / kKeys - t0);
-    k0 = t0 + static_cast<int>(static_cast<int64_t>(n) * span / ta.spans);
-    k1 = t0 + static_cast<int>(static_cast<int64_t>(n) * (span + 1) / ta.spans);
+    k0 = t0 + static_cast<int>(static_cast<int64_t>(n) * span / spans);
+    k1 = t0 + static_cast<int>(static_cast<int64_t>(n) * (span + 1) / spans);
   }
   const int n_tiles = k1 - k0;
   // (not zero: a score that is masked by -inf stays so times it)
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     auto rows_of = [&](int t) {
       Rows x{{0, 0}, kIts, {0, 0}};
       const int j = (k0 + t) * kKeys + row0, n = min(r.kv_len - j, n_rows);
-      if (n <= 0) return x;
+      if (n <= 0 || t >= n_tiles) return x;
       const int off = j & mask;
       x.turn = min(kIts, mask + 1 - off);
       if (two_pages) {
@@ -917,10 +944,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const int64_t at = static_cast<int64_t>(r.start + tok) * a.q_heads + h * a.group + hh;
       const float up = BITS == 16 ? 1.f : exp2f(static_cast<float>(e_now));  // 2^E
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const int part = same_rows ? 2 * span + chain : span;
-      const int64_t slot = ((static_cast<int64_t>(tile) * a.kv.kv_heads + h) * max(ta.parts, 1) + part) * ta.tile_rows + my_row;
-      if (in && ta.parts > 0) ta.ml[slot] = make_float2(ref, l);
-      if (in && ta.parts == 0 && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * kLn2;
+      const bool cut = ta.cut(shares, block);
+      const int64_t slot = cut ? static_cast<int64_t>(ta.slot(shares, block) + (same_rows ? chain : 0)) * ta.tile_rows + my_row : 0;
+      if (in && cut) ta.ml[slot] = make_float2(ref, l);
+      if (in && !cut && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * kLn2;
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         float x[16];
@@ -939,7 +966,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           for (int e = 0; e < 16; ++e) x[e] = 0.f;
         }
         if (!in) continue;
-        if (ta.parts > 0) {
+        if (cut) {
           float4* const dst = reinterpret_cast<float4*>(ta.o + slot * DP + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
@@ -956,45 +983,48 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   }
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const int64_t at = (work ? (static_cast<int64_t>(tile) * a.kv.kv_heads + h) * ta.spans + span : blockIdx.x);
-    ta.note[at] = TileNote{r.start, row0, rows, h, b, *s_odd};
-  }
+  if (threadIdx.x == 0) ta.note[block] = TileNote{r.start, row0, rows, h, b, *s_odd};
   if (warp == kMmaWarp) tmem_dealloc(tmem, K::kCols);
 }
 
-// Adds up a tile's parts, eight rows (four of 256 columns) a step; and, where a value that
-// is no number met rows that do not see it, takes the tile's rows one by one.
+// Adds up the parts of items that were cut, a few rows of one at a time; and, where a
+// value that is no number met rows that do not see it, takes an item's rows one by one.
 constexpr int kJoinThreads = 128;
 template <typename T, int BITS, int DP>
 __global__ void __launch_bounds__(kJoinThreads) k_attn_tiles(const AttnArgs a, const TileArgs ta) {
   __shared__ AttnRowSmem sm;
   constexpr int kCols = DP / 4, kGroups = kJoinThreads / kCols;
   grid_dep_wait();
-  const int64_t which = blockIdx.x;
-  const TileNote note = ta.note[which * ta.spans];
-  if (note.rows <= 0) return;
-  if constexpr (BITS == 16) {
+  const Shares shares = *ta.shares;
+  const int chains = ta.tile_rows == kRows ? 2 : 1;
+  auto first_block = [&](int item) {
+    return item < shares.whole ? item : shares.whole + (item - shares.whole) * shares.spans;
+  };
+  auto is_odd = [&](int item) {
     bool odd = false;
-    for (int s = 0; s < ta.spans; ++s) odd |= ta.note[which * ta.spans + s].odd != 0;
-    if (odd) {
-      const SeqRange r = seq_range(a, note.seq);
-      for (int row = blockIdx.y; row < note.rows; row += gridDim.y)
-        attn_one_row<T, BITS>(a, note.seq, r, (note.row0 + row) / a.group, note.head * a.group + (note.row0 + row) % a.group, sm);
-      return;
+    if constexpr (BITS == 16) {
+      const int i = first_block(item);
+      for (int s = 0; s < (item < shares.whole ? 1 : shares.spans); ++s) odd |= ta.note[i + s].odd != 0;
     }
-  }
-  if (ta.parts == 0) return;
+    return odd;
+  };
+  const int steps = ta.tile_rows / kGroups;  // of kGroups rows an item
+  const int first = chains == 2 ? 0 : shares.spans > 1 ? shares.whole : shares.items;
   const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
-  for (int row = blockIdx.y * kGroups + grp; row < note.rows; row += gridDim.y * kGroups) {
-    const int64_t s0 = which * ta.parts * ta.tile_rows + row;
+  for (int64_t u = blockIdx.x; u < static_cast<int64_t>(shares.items - first) * steps; u += gridDim.x) {
+    const int item = first + static_cast<int>(u / steps);
+    const int i = first_block(item), parts = chains * (item < shares.whole ? 1 : shares.spans);
+    const TileNote note = ta.note[i];
+    const int row = static_cast<int>(u % steps) * kGroups + grp;
+    if (row >= note.rows || is_odd(item)) continue;
+    const int64_t s0 = static_cast<int64_t>(ta.slot(shares, i)) * ta.tile_rows + row;
     float top = -INFINITY;
-    for (int p = 0; p < ta.parts; ++p) top = fmaxf(top, ta.ml[s0 + static_cast<int64_t>(p) * ta.tile_rows].x);
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, ta.ml[s0 + static_cast<int64_t>(p) * ta.tile_rows].x);
     const float ref = top == -INFINITY ? 0.f : top;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < ta.parts; ++p) {
+    for (int p = 0; p < parts; ++p) {
       const int64_t s = s0 + static_cast<int64_t>(p) * ta.tile_rows;
       const float2 ml = ta.ml[s];
       const float4 v = *reinterpret_cast<const float4*>(ta.o + s * DP + col * 4);
@@ -1016,23 +1046,32 @@ __global__ void __launch_bounds__(kJoinThreads) k_attn_tiles(const AttnArgs a, c
     }
     if (col == 0 && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
   }
+  if constexpr (BITS == 16) {
+    for (int item = blockIdx.x; item < shares.items; item += gridDim.x) {
+      if (!is_odd(item)) continue;
+      const TileNote note = ta.note[first_block(item)];
+      const SeqRange r = seq_range(a, note.seq);
+      for (int row = 0; row < note.rows; ++row)
+        attn_one_row<T, BITS>(a, note.seq, r, (note.row0 + row) / a.group, note.head * a.group + (note.row0 + row) % a.group, sm);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ host
 struct Plan {
-  int tile_rows, spans, parts;
-  int64_t tiles;  // at most
+  int tile_rows, most_spans, blocks, slots;
 };
 Plan plan(const AttnArgs& a, int max_q_len, int max_kv_len) {
   Plan p;
+  const int sms = device_sm_count();
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.group;
   p.tile_rows = static_cast<int64_t>(max_q_len) * a.group <= kRows ? kRows : 2 * kRows;
-  p.tiles = std::min<int64_t>(rows, rows / p.tile_rows + a.num_seqs);  // a partial one each
-  const int64_t blocks = p.tiles * a.kv.kv_heads;
-  // spans until the blocks fill the machine, none shorter than 512 keys
-  const int64_t most = std::max<int64_t>(1, max_kv_len / 512);
-  p.spans = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(device_sm_count() / std::max<int64_t>(1, blocks), most)));
-  p.parts = p.tile_rows == kRows ? 2 * p.spans : p.spans > 1 ? p.spans : 0;
+  const int64_t tiles = std::min<int64_t>(rows, rows / p.tile_rows + a.num_seqs);  // a partial one each
+  // an item may be cut until a part has 512 keys
+  p.most_spans = std::max(1, max_kv_len / 512);
+  // whole rounds of items, and a round of parts
+  p.blocks = static_cast<int>(tiles * a.kv.kv_heads / sms * sms + sms);
+  p.slots = p.tile_rows == kRows ? 2 * p.blocks : sms;
   return p;
 }
 size_t round256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -1067,31 +1106,32 @@ bool cache_map(CUtensorMap* m, const KvDev& kv, const void* base, bool bf16) {
 template <typename T, int BITS, int DP>
 struct Many {
   static std::atomic<size_t> raised[kMaxDevices];
-  static size_t workspace(const AttnArgs& a, const Plan& p) {
-    const size_t heads = static_cast<size_t>(p.tiles) * a.kv.kv_heads;
-    return round256(heads * p.spans * sizeof(TileNote)) +
-           heads * p.parts * p.tile_rows * (DP * sizeof(float) + sizeof(float2));
+  static size_t workspace(const Plan& p) {
+    return round256(sizeof(Shares)) + round256(p.blocks * sizeof(TileNote)) +
+           static_cast<size_t>(p.slots) * p.tile_rows * (DP * sizeof(float) + sizeof(float2));
   }
   static cudaError_t launch(const AttnArgs& a, const Plan& p, void* ws, cudaStream_t s) {
     using K = Tc<T, BITS, DP>;
     cudaError_t e = raise_smem_limit(k_attn_many<T, BITS, DP>, K::kSmem, raised);
     if (e != cudaSuccess) return e;
-    const size_t heads = static_cast<size_t>(p.tiles) * a.kv.kv_heads;
     TileArgs ta;
-    ta.note = static_cast<TileNote*>(ws);
-    ta.o = reinterpret_cast<float*>(static_cast<char*>(ws) + round256(heads * p.spans * sizeof(TileNote)));
-    ta.ml = reinterpret_cast<float2*>(ta.o + heads * p.parts * p.tile_rows * DP);
-    ta.spans = p.spans;
-    ta.parts = p.parts;
+    char* w = static_cast<char*>(ws);
+    ta.shares = reinterpret_cast<Shares*>(w);
+    w += round256(sizeof(Shares));
+    ta.note = reinterpret_cast<TileNote*>(w);
+    w += round256(p.blocks * sizeof(TileNote));
+    ta.o = reinterpret_cast<float*>(w);
+    ta.ml = reinterpret_cast<float2*>(ta.o + static_cast<size_t>(p.slots) * p.tile_rows * DP);
+    ta.sms = device_sm_count();
+    ta.most_spans = p.most_spans;
     ta.tile_rows = p.tile_rows;
     CUtensorMap maps[2] = {};
     ta.tma = BITS == 16 && cache_map(&maps[0], a.kv, a.kv.k, std::is_same_v<T, __nv_bfloat16>) &&
              cache_map(&maps[1], a.kv, a.kv.v, std::is_same_v<T, __nv_bfloat16>);
-    e = launch_dep(k_attn_many<T, BITS, DP>, dim3(static_cast<unsigned>(heads * p.spans)), dim3(kThreads), K::kSmem, s, a, ta,
-                   maps[0], maps[1]);
-    if (e != cudaSuccess || (BITS != 16 && p.parts == 0)) return e;
-    return launch_dep(k_attn_tiles<T, BITS, DP>, dim3(static_cast<unsigned>(heads), p.parts > 0 ? 32u : 1u), dim3(kJoinThreads), 0,
-                      s, a, ta);
+    e = launch_dep(k_attn_many<T, BITS, DP>, dim3(static_cast<unsigned>(p.blocks)), dim3(kThreads), K::kSmem, s, a, ta, maps[0],
+                   maps[1]);
+    if (e != cudaSuccess) return e;
+    return launch_dep(k_attn_tiles<T, BITS, DP>, dim3(static_cast<unsigned>(8 * ta.sms)), dim3(kJoinThreads), 0, s, a, ta);
   }
 };
 template <typename T, int BITS, int DP>
@@ -1123,7 +1163,7 @@ cudaError_t take_many_error(uint32_t* code) {
 
 size_t many_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len) {
   const Plan p = plan(a, max_q_len, max_kv_len);
-  return with_many(bits, bf16, a.kv.head_dim, [&](auto k) { return decltype(k)::workspace(a, p); });
+  return with_many(bits, bf16, a.kv.head_dim, [&](auto k) { return decltype(k)::workspace(p); });
 }
 cudaError_t launch_many(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
                         cudaStream_t s) {
