@@ -161,3 +161,13 @@ def test_plain_forms_agree_with_themselves():
     assert tokens.tolist() == [[2, 2, 2]] and accepted.tolist() == [2]
     tokens, accepted, _, _ = verify_plain(logits, drafts, np.array([[0.0, 0.9999]]), noise)
     assert accepted.tolist() == [1] and tokens[0, 1] != 2 and tokens[0, 2] == -1
+
+
+def test_lookup_draft_finds_the_latest_continuation():
+    from robustgemq_b200.inference.speculative import lookup_draft
+
+    assert lookup_draft([1, 2, 3, 9, 1, 2, 3, 4, 5, 1, 2, 3], 2) == [4, 5]
+    assert lookup_draft([1, 2, 3, 9, 1, 2, 3], 10) == [9, 1, 2, 3]
+    assert lookup_draft([5, 6, 7, 6], 3) == [7, 6]
+    assert lookup_draft([1, 2, 3], 3) == [] and lookup_draft([1], 3) == [] and lookup_draft([], 3) == []
+    assert lookup_draft([4, 4], 0) == []
