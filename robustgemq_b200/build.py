@@ -23,6 +23,9 @@ LIB = PKG / "libgemq_b200.so"
 SOURCES = ["gemq_api.cu", "kernels_misc.cu", "kernels_route.cu", "kernels_decode.cu", "kernels_tc.cu",
            "kernels_tcd.cu", "kernels_simt.cu", "kernels_cache.cu", "kernels_attn.cu", "kernels_attn_tc.cu", "kernels_verify.cu",
            "serving_api.cu"]
+# the torch binding of the serving operators
+EXT = PKG / "_serving_ext.so"
+EXT_SOURCE = "serving_ext.cpp"
 HEADERS = ["gemq_common.cuh", "gemq_internal.h", "tc_work.cuh", "kperm.cuh", "paged.cuh", "attn_rows.cuh"]
 # compiled without relocatable device code: ptxas ignores setmaxnreg with it
 WHOLE = {"kernels_attn_tc.cu"}
@@ -44,9 +47,50 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def _ext_stale() -> bool:
+    if not EXT.exists():
+        return True
+    t = EXT.stat().st_mtime
+    return any(p.stat().st_mtime > t for p in (CSRC / EXT_SOURCE, ROOT / "include" / "gemq_b200.h"))
+
+
+def _ext_commands(obj: Path):
+    """Compile and link commands of the torch binding (host code only)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = [*cpp_extension.include_paths(device_type="cuda"), sysconfig.get_paths()["include"]]
+    compile_cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                   "-DTORCH_EXTENSION_NAME=_serving_ext", *[f"-I{p}" for p in includes], "-c", str(CSRC / EXT_SOURCE),
+                   "-o", str(obj)]
+    libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+    link_cmd = ["g++", "-shared", "-o", str(EXT.with_suffix(".so.tmp")), str(obj), f"-L{PKG}", "-l:libgemq_b200.so",
+                "-Wl,-rpath,$ORIGIN", *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    return compile_cmd, link_cmd
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
-    if not force and not _stale():
-        return LIB
+    """Builds the library and, beside it, the torch binding of the serving operators."""
+    ext = None
+    if force or _ext_stale():
+        objdir = ROOT / "_build"
+        objdir.mkdir(exist_ok=True)
+        compile_cmd, link_cmd = _ext_commands(objdir / "serving_ext.o")
+        ext = subprocess.Popen(compile_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if force or _stale():
+        _build_lib(verbose, jobs)
+    if ext is not None:
+        _wait((EXT_SOURCE, ext), verbose)
+        out = subprocess.run(link_cmd, capture_output=True, text=True)
+        if out.returncode != 0:
+            raise RuntimeError(f"link failed:\n{out.stdout}\n{out.stderr}")
+        os.replace(EXT.with_suffix(".so.tmp"), EXT)
+    return LIB
+
+
+def _build_lib(verbose: bool, jobs: int) -> Path:
     nvcc = nvcc_path()
     objdir = ROOT / "_build"
     objdir.mkdir(exist_ok=True)
@@ -78,7 +122,7 @@ def _wait(item, verbose):
     src, proc = item
     out, _ = proc.communicate()
     if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed on {src}:\n{out}")
+        raise RuntimeError(f"compiler failed on {src}:\n{out}")
     if verbose and out:
         sys.stdout.write(f"--- {src}\n{out}")
 

@@ -5,6 +5,7 @@ Bounds are derived in ``serving_helpers`` from the operations' roundings."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -293,7 +294,7 @@ def test_attention_leaves_tokens_outside_every_sequence():
     out = torch.full_like(q, 7.0)
     ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
     _lib.check(lib.gemq_paged_attention(
-        b.cache._ref, q.data_ptr(), q.stride(0), 8, 2, b.page_table.data_ptr(), b.page_table.stride(0),
+        ctypes.cast(b.cache.c_struct, ctypes.POINTER(_lib.KvCacheT)), q.data_ptr(), q.stride(0), 8, 2, b.page_table.data_ptr(), b.page_table.stride(0),
         b.page_table.shape[1], b.kv_lens.data_ptr(), b.q_starts.data_ptr(), 2, 3, 50, 0.125, 0, out.data_ptr(), None,
         ws.data_ptr(), ws.numel(), _lib.stream_ptr(q.device)))
     o, _, tol, _ = b.expect(0.125)
