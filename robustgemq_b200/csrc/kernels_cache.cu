@@ -27,28 +27,27 @@ namespace {
 constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 
-// How a warp takes rows: a row is D / 8 chunks of eight elements, a lane takes two of them,
-// half a row apart, so G = ceil(D / 16) lanes a row and 32 / G rows a warp, whatever D. The
-// lanes of a chunk's half are neighbours in memory in every form.
+// How a warp takes rows: a lane takes two chunks of eight elements, half a row apart, so
+// G = D / 16 lanes a row and 32 / G rows a warp (D is a multiple of 16). The lanes of a
+// half are neighbours in memory in every form.
 struct Lanes {
   int g, rows;      // lanes a row, rows a warp
   uint32_t inv_g;   // floor(65536 / g) + 1: l / g = l inv_g >> 16 for l < 32
 };
 Lanes lanes_of(int head_dim) {
-  const int g = (head_dim / 8 + 1) / 2;
+  const int g = head_dim / 16;
   return {g, 32 / g, 65536u / static_cast<uint32_t>(g) + 1u};
 }
 struct Lane {
-  int row, sub;     // of the warp's rows; of the row's lanes
-  bool first, second;  // whether its chunks are there
+  int row, sub;  // of the warp's rows; of the row's lanes
+  bool has_row;  // the last 32 % G lanes have none
 };
-__device__ __forceinline__ Lane lane_of(const Lanes& l, int head_dim) {
+__device__ __forceinline__ Lane lane_of(const Lanes& l) {
   const int lane = threadIdx.x & 31;
   Lane x;
   x.row = static_cast<int>(static_cast<uint32_t>(lane) * l.inv_g >> 16);
   x.sub = lane - x.row * l.g;
-  x.first = x.row < l.rows;
-  x.second = x.first && (x.sub + l.g) * 8 < head_dim;
+  x.has_row = x.row < l.rows;
   return x;
 }
 
@@ -164,7 +163,7 @@ __global__ void __launch_bounds__(kRowThreads, 8) k_cache_write(const KvDev c, c
                                                             const int64_t* __restrict__ slots, uint32_t rows,
                                                             HeadDiv div, Lanes lanes) {
   using T2 = typename Vec2<T>::type;
-  const Lane me = lane_of(lanes, c.head_dim);
+  const Lane me = lane_of(lanes);
   const uint32_t r0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * static_cast<uint32_t>(U * lanes.rows) + me.row;
   const int64_t total = static_cast<int64_t>(c.num_pages) << c.page_shift;
   grid_dep_wait();
@@ -175,15 +174,15 @@ __global__ void __launch_bounds__(kRowThreads, 8) k_cache_write(const KvDev c, c
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t r = r0 + u * lanes.rows;
-    const bool live = me.first && r < 2 * rows;
+    const bool live = me.has_row && r < 2 * rows;
     id[u] = row_id(live ? r : 0u, rows, static_cast<uint32_t>(c.kv_heads), div);
     slot[u] = -1;
-    raw[u][0] = make_uint4(0, 0, 0, 0);
+    raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
     if (live) {
       slot[u] = __ldg(slots + id[u].token);
       const T* src = id[u].v ? v + id[u].token * v_ts + id[u].head * v_hs : k + id[u].token * k_ts + id[u].head * k_hs;
       raw[u][0] = __ldcs(reinterpret_cast<const uint4*>(src + me.sub * 8));
-      if (me.second) raw[u][1] = __ldcs(reinterpret_cast<const uint4*>(src + (me.sub + lanes.g) * 8));
+      raw[u][1] = __ldcs(reinterpret_cast<const uint4*>(src + (me.sub + lanes.g) * 8));
     }
   }
 #pragma unroll
@@ -193,10 +192,11 @@ __global__ void __launch_bounds__(kRowThreads, 8) k_cache_write(const KvDev c, c
     const uint32_t at = put ? static_cast<uint32_t>(slot[u]) : 0u;
     uint8_t* dst = (id[u].v ? c.v : c.k) + slot_row(c, at, id[u].head) + me.sub * BITS;
     if constexpr (BITS == 16) {
-      if (put) *reinterpret_cast<uint4*>(dst) = raw[u][0];
-      if (put && me.second) *reinterpret_cast<uint4*>(dst + lanes.g * BITS) = raw[u][1];
+      if (put) {
+        *reinterpret_cast<uint4*>(dst) = raw[u][0];
+        *reinterpret_cast<uint4*>(dst + lanes.g * BITS) = raw[u][1];
+      }
     } else {
-      if (!me.second) raw[u][1] = raw[u][0];  // for the extremes
       // (max |x|, the same) or (max x, max -x) of the row
       T2 top;
       {
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kRowThreads, 8) k_cache_write(const KvDev c, c
       if (poison) w0 = w1 = make_uint2(0, 0);
       if (put) {
         put_codes<BITS>(dst, w0);
-        if (me.second) put_codes<BITS>(dst + lanes.g * BITS, w1);
+        put_codes<BITS>(dst + lanes.g * BITS, w1);
         if (me.sub == 0) {
           float* s = (id[u].v ? c.v_scale : c.k_scale) + slot_scale(c, at, id[u].head);
           const float step = poison ? NAN : __fdiv_rn(range, kTop);
@@ -306,12 +306,12 @@ template <typename T, int BITS, int U>
 __global__ void __launch_bounds__(kRowThreads) k_cache_read(const KvDev c, const int64_t* __restrict__ slots,
                                                            uint32_t rows, HeadDiv div, Lanes lanes, T* __restrict__ k,
                                                            T* __restrict__ v) {
-  const Lane me = lane_of(lanes, c.head_dim);
+  const Lane me = lane_of(lanes);
   const uint32_t r0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * static_cast<uint32_t>(U * lanes.rows) + me.row;
   const int64_t total = static_cast<int64_t>(c.num_pages) << c.page_shift;
   grid_dep_wait();
   grid_dep_launch();
-  if (!me.first) return;
+  if (!me.has_row) return;
   RowId id[U];
   bool live[U];
   uint4 raw[U][2];
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cache_read(const KvDev c, const
       const uint32_t at = static_cast<uint32_t>(slot[u]);
       const uint8_t* src = (id[u].v ? c.v : c.k) + slot_row(c, at, id[u].head) + me.sub * BITS;
       raw[u][0] = get_codes<BITS>(src);
-      if (me.second) raw[u][1] = get_codes<BITS>(src + lanes.g * BITS);
+      raw[u][1] = get_codes<BITS>(src + lanes.g * BITS);
       if constexpr (BITS != 16) {
         const float* s = (id[u].v ? c.v_scale : c.k_scale) + slot_scale(c, at, id[u].head);
         if constexpr (BITS == 8) sc[u].x = *s;
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cache_read(const KvDev c, const
     }
     T* dst = (id[u].v ? v : k) + (static_cast<int64_t>(id[u].token) * c.kv_heads + id[u].head) * c.head_dim + me.sub * 8;
     __stcs(reinterpret_cast<uint4*>(dst), out[0]);
-    if (me.second) __stcs(reinterpret_cast<uint4*>(dst + lanes.g * 8), out[1]);
+    __stcs(reinterpret_cast<uint4*>(dst + lanes.g * 8), out[1]);
   }
 }
 
