@@ -1053,22 +1053,24 @@ int most_rows(const AttnArgs& a, int max_q_len) {
   return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(max_q_len) * a.group, 1 << 20));
 }
 
-// More rows a KV head than kFewRows go to the tensor-memory kernel.
-constexpr int kFewRows = 32;
-bool takes_many(const AttnArgs& a, int max_q_len) {
-  return most_rows(a, max_q_len) > kFewRows && a.kv.head_dim <= 128;
+// More rows a KV head than this go to the tensor-memory kernel. Above 128 columns its
+// loaders' unpacking serves 128 rows only, so that codes take more rows to pay (16
+// sequences of 3,000, 36 rows a KV head x 256: 16 bits 68 us there against 141 here, 8 bits
+// 161 against 133).
+bool takes_many(const AttnArgs& a, int bits, int max_q_len) {
+  return most_rows(a, max_q_len) > (bits != 16 && a.kv.head_dim > 128 ? 64 : 32);
 }
 
 }  // namespace
 
 size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len) {
-  if (takes_many(a, max_q_len)) return many_workspace(a, bits, bf16, max_q_len, max_kv_len);
+  if (takes_many(a, bits, max_q_len)) return many_workspace(a, bits, bf16, max_q_len, max_kv_len);
   return with_few(bits, bf16, a.kv.head_dim, most_rows(a, max_q_len), [&](auto k) { return decltype(k)::workspace(); });
 }
 
 cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
                              cudaStream_t s) {
-  if (takes_many(a, max_q_len)) return launch_many(a, bits, bf16, max_q_len, max_kv_len, workspace, s);
+  if (takes_many(a, bits, max_q_len)) return launch_many(a, bits, bf16, max_q_len, max_kv_len, workspace, s);
   const int rows = most_rows(a, max_q_len);
   return with_few(bits, bf16, a.kv.head_dim, rows, [&](auto k) { return decltype(k)::launch(a, rows, workspace, s); });
 }

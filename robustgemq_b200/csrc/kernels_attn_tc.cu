@@ -30,6 +30,12 @@
 // Row tiles that do not fill a last round of the machine (all of them, where they are few)
 // are cut along their keys until they do, and k_attn_tiles adds the parts up; with at most
 // 128 rows a KV head both chains take the same rows and every second tile of keys each.
+// Above 128 columns the sums of 256 rows would fill tensor memory: both chains take the
+// same 128 rows and all keys, 64 at a time, and half of V's columns each. S and P are formed
+// twice, so two of six products are repeated, but Q and the keys stand in shared memory
+// once, and all else stays as it is. (2,048 tokens at the end of 8,192, 16 query and 4 KV
+// heads x 256: 334 us, 720 TFLOP/s, at 16 bits, where 16-row tiles took 3,141; 819 and 890
+// at 8 and 4 bits, the loaders' unpacking, against 2,810 and 1,683.)
 //
 // Measured on a B200: 4,096 tokens at the end of 16,384, 32 query and 8 KV heads x 128,
 // bf16: 890 us (1,080 TFLOP/s of the visible pairs; 1,020 us in long runs under the power
@@ -54,28 +60,30 @@ constexpr int kMmaWarp = 8;       // and 9
 constexpr int kLoadWarp = 12;
 constexpr int kLoaders = 128;
 constexpr int kThreads = 32 * (kLoadWarp + 4);
-// Registers after the split: 256 x 184 + 256 x 72 = 512 x 128, what the block starts with.
-constexpr int kSoftRegs = 184, kOtherRegs = 72;
-static_assert(256 * (kSoftRegs + kOtherRegs) <= kThreads * 128, "more registers than the block was launched with");
 constexpr float kSlack = 8.f;     // how far a score may pass the reference, in powers of two
 
 template <typename T, int BITS, int DP>
 struct Tc {
-  static constexpr int kKeys = DP == 64 ? 128 : 80;  // of a tile
+  static constexpr bool kWide = DP == 256;           // each chain half of the columns of V
+  static constexpr int kKeys = DP == 64 ? 128 : DP == 128 ? 80 : 64;  // of a tile
   static constexpr int kPanels = DP / 64;            // of 64 columns (128 bytes) each
   static constexpr int kPanel = kKeys * 128;         // bytes
   static constexpr int kTile = kPanels * kPanel;     // K tile, V tile
   static constexpr int kQPanel = kRows * 128;
   static constexpr int kQTile = kPanels * kQPanel;
-  static constexpr int kStages = 6;                  // K and V in turn
+  static constexpr int kStages = kWide ? 4 : 6;      // K and V in turn
   static constexpr int kQOff = 0;
-  static constexpr int kRingOff = 2 * kQTile;
+  static constexpr int kRingOff = (kWide ? 1 : 2) * kQTile;
   static constexpr int kPrepOff = kRingOff + kStages * kTile;   // per key factors, two tiles
   static constexpr int kPrepTile = BITS == 16 ? 0 : (BITS == 8 ? 2 : 4) * kKeys * 4;
   static constexpr int kBarOff = kPrepOff + 2 * kPrepTile;
   static constexpr int kBars = 2 * kStages + 16;
   static constexpr int kSmem = kBarOff + kBars * 8 + 128 + 1024;  // + alignment
   static_assert(kSmem <= 227 * 1024, "shared memory");
+  // Registers after the split: 256 x (184 + 72) = 512 x 128, what the block starts with (a
+  // tile of 64 keys is less to hold, and its rows of 256 columns more to have on the way).
+  static constexpr int kSoftRegs = kWide ? 160 : 184, kOtherRegs = kWide ? 96 : 72;
+  static_assert(256 * (kSoftRegs + kOtherRegs) <= kThreads * 128, "more registers than the block was launched with");
   using C = std::conditional_t<BITS == 16, T, __half>;
   static constexpr bool kRowFactor = BITS != 16 && std::is_same_v<T, __nv_bfloat16>;
   static constexpr uint32_t kType = std::is_same_v<C, __nv_bfloat16> ? 1u : 0u;
@@ -83,8 +91,11 @@ struct Tc {
   static constexpr int kCols = 512;
   static constexpr int kOCol = DP == 64 ? 384 : 256;
   __device__ static constexpr uint32_t s_at(int i) { return i * 128; }
-  __device__ static constexpr uint32_t p_at(int i) { return DP == 64 ? 256 + i * 64 : i * 128 + 80; }
-  __device__ static constexpr uint32_t o_at(int i) { return kOCol + i * DP; }
+  __device__ static constexpr uint32_t p_at(int i) { return DP == 64 ? 256 + i * 64 : i * 128 + kKeys; }
+  __device__ static constexpr uint32_t o_at(int i) { return kOCol + i * (kWide ? 128 : DP); }
+  // the columns of V, and of the output, that are chain i's: a number of them from the first
+  __device__ static constexpr int first_col(int i) { return kWide ? i * 128 : 0; }
+  __device__ static constexpr int num_cols(int i, int head_dim) { return !kWide ? head_dim : i == 0 ? 128 : head_dim - 128; }
   static_assert(DP == 64 || kKeys + kKeys / 2 <= 128, "S and P of a chain in 128 columns");
 };
 
@@ -205,6 +216,7 @@ struct TileArgs {
   int sms;
   int most_spans;  // of an item
   int tile_rows;   // 256; 128 where both chains take the same rows
+  bool alternate;  // they take every second tile of keys each
   bool tma;        // the maps of the cache are valid (16 bits, pages of 16 tokens and more)
 
   __device__ __forceinline__ Shares share(int items) const {
@@ -216,10 +228,10 @@ struct TileArgs {
   }
   // the first slot of block i's parts (one, or a chain each)
   __device__ __forceinline__ int slot(const Shares& s, int i) const {
-    return tile_rows == kRows ? 2 * i : i - s.whole;
+    return alternate ? 2 * i : i - s.whole;
   }
   __device__ __forceinline__ bool cut(const Shares& s, int i) const {
-    return tile_rows == kRows || (i >= s.whole && s.spans > 1);
+    return alternate || (i >= s.whole && s.spans > 1);
   }
 };
 
@@ -250,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   int* const s_e = s_exp + 8;                   // [2] E of the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.kv.head_dim;
-  const bool same_rows = ta.tile_rows == kRows;
+  const bool alternate = !K::kWide && ta.alternate, same_rows = K::kWide || alternate;
 
   if (warp == kMmaWarp) {
     tmem_alloc(s_tmem, K::kCols);
@@ -317,13 +329,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   const float cs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
 
   // which tiles chain i takes: all, or every second one
-  const int step = same_rows ? 2 : 1;
-  auto chain_first = [&](int i) { return same_rows ? i : 0; };
+  const int step = alternate ? 2 : 1;
+  auto chain_first = [&](int i) { return alternate ? i : 0; };
   // a chain without rows is left out
   const bool chain_b = same_rows || rows > kRows;
 
   if (threadIdx.x == 0) {
-    const int chains = chain_b && !same_rows ? 2 : 1;  // that take each tile
+    const int chains = chain_b && !alternate ? 2 : 1;  // that take each tile
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 4);  // one arrival a loader warp
       mbar_init(&empty[s], chains);
@@ -377,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       rf = exp2f(static_cast<float>(e));
       inv_factor = 1.f / rf;
     }
-    uint8_t* const dst = smem + K::kQOff + chain * K::kQTile + tid * 128;
+    uint8_t* const dst = smem + K::kQOff + (K::kWide ? 0 : chain * K::kQTile) + tid * 128;
 #pragma unroll 4
     for (int c = 0; c < D / 8; ++c) {
       uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -407,7 +419,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           qsum += f.x + f.y;
         }
       }
-      *reinterpret_cast<uint4*>(dst + (c >> 3) * K::kQPanel + (((c & 7) ^ (tid & 7)) << 4)) = w;
+      if (!K::kWide || chain == 0)
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * K::kQPanel + (((c & 7) ^ (tid & 7)) << 4)) = w;
     }
     fence_proxy_async_smem();
   }
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
 
   bool ok = true;  // no wait of this thread ran out
   if (warp >= kLoadWarp) {
-    regs_down<kOtherRegs>();
+    regs_down<K::kOtherRegs>();
     // ---------------------------------------------------------- loads
     const int me = static_cast<int>(threadIdx.x) - kLoadWarp * 32;
     const int mask = (1 << a.kv.page_shift) - 1;
@@ -714,12 +727,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     }
   } else if (warp >= kMmaWarp) {
     // ---------------------------------------------------------- products of one chain
-    regs_down<kOtherRegs>();
+    regs_down<K::kOtherRegs>();
     const int i = warp - kMmaWarp;
     if (i == 0 || (i == 1 && chain_b)) {
       const uint32_t s_col = tmem + K::s_at(i), p_col = tmem + K::p_at(i), o_col = tmem + K::o_at(i);
-      const uint32_t id_s = idesc(K::kType, kKeys, false), id_o = idesc(K::kType, D, true);
-      const uint32_t q_addr = smem_u32(smem + K::kQOff + i * K::kQTile);
+      const uint32_t id_s = idesc(K::kType, kKeys, false), id_o = idesc(K::kType, K::num_cols(i, D), true);
+      const uint32_t q_addr = smem_u32(smem + K::kQOff + (K::kWide ? 0 : i * K::kQTile));
       const int ks = D / 16;
       // S of tile t, once its keys are there
       auto product_s = [&](int t) {
@@ -753,10 +766,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t v = sdesc_v(smem_u32(smem + K::kRingOff + s * K::kTile), K::kPanel);
+          const uint64_t v = sdesc_v(smem_u32(smem + K::kRingOff + s * K::kTile + K::first_col(i) / 64 * K::kPanel), K::kPanel);
           umma_pv(o_col, p_col, v, id_o, n > 0);
           if constexpr (kKeys == 128) umma_pv(o_col, p_col + 32, v + 512, id_o, 1);
-          else umma_f16_ts(o_col, p_col + 32, v + 512, id_o, 1);
+          if constexpr (kKeys == 80) umma_f16_ts(o_col, p_col + 32, v + 512, id_o, 1);
           umma_commit(&o_done[i]);
           umma_commit(&empty[s]);
         }
@@ -767,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       mbar_wait_drain(&drain[i], 0);
     }
   } else {
-    regs_up<kSoftRegs>();
+    regs_up<K::kSoftRegs>();
     if (chain == 0 || chain_b) {
     // ---------------------------------------------------------- softmax: a thread a row
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp
@@ -777,6 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     const int w_row = my_row - lane;
     const int w_min = pos0 + (row0 + w_row) / a.group;
     const int w_max = pos0 + (row0 + min(w_row + 31, max(rows, 1) - 1)) / a.group;
+    const int cols = K::num_cols(chain, D);
     float ref = -INFINITY, l = 0.f, zacc = 0.f;
     int e_now = -126;  // E of the sums so far
     int n = 0;
@@ -849,7 +863,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = 0; c < cols; c += 16) {
             uint32_t o[16];
             tmem_ld16(o_col + c, o);
             tmem_ld_wait();
@@ -902,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       tmem_st32(p_col, reinterpret_cast<uint32_t(&)[32]>(p[0]));
       weights(32, kKeys / 2);
       if constexpr (kKeys == 128) tmem_st32(p_col + 32, reinterpret_cast<uint32_t(&)[32]>(p[32]));
-      else tmem_st8(p_col + 32, reinterpret_cast<uint32_t(&)[8]>(p[32]));
+      if constexpr (kKeys == 80) tmem_st8(p_col + 32, reinterpret_cast<uint32_t(&)[8]>(p[32]));
       {
         float x0, x1, y0, y1;
         split(lt[0], x0, x1);
@@ -926,11 +940,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const float up = BITS == 16 ? 1.f : exp2f(static_cast<float>(e_now));  // 2^E
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       const bool cut = ta.cut(shares, block);
-      const int64_t slot = cut ? static_cast<int64_t>(ta.slot(shares, block) + (same_rows ? chain : 0)) * ta.tile_rows + my_row : 0;
-      if (in && cut) ta.ml[slot] = make_float2(ref, l);
-      if (in && !cut && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * kLn2;
+      const int64_t slot = cut ? static_cast<int64_t>(ta.slot(shares, block) + (alternate ? chain : 0)) * ta.tile_rows + my_row : 0;
+      const bool tells = in && (!K::kWide || chain == 0);  // the row's sums, which both have
+      if (tells && cut) ta.ml[slot] = make_float2(ref, l);
+      if (tells && !cut && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * kLn2;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
+      for (int c = 0; c < cols; c += 16) {
         float x[16];
         if (n > 0) {
           uint32_t o[16];
@@ -948,11 +963,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         }
         if (!in) continue;
         if (cut) {
-          float4* const dst = reinterpret_cast<float4*>(ta.o + slot * DP + c);
+          float4* const dst = reinterpret_cast<float4*>(ta.o + slot * DP + K::first_col(chain) + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
         } else {
-          uint4* const dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at * D + c);
+          uint4* const dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at * D + K::first_col(chain) + c);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             dst[e] = make_uint4(pack2<T>(x[8 * e] * inv, x[8 * e + 1] * inv), pack2<T>(x[8 * e + 2] * inv, x[8 * e + 3] * inv),
@@ -977,7 +992,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attn_tiles(const AttnArgs a, c
   constexpr int kCols = DP / 4, kGroups = kJoinThreads / kCols;
   grid_dep_wait();
   const Shares shares = *ta.shares;
-  const int chains = ta.tile_rows == kRows ? 2 : 1;
+  const int chains = ta.alternate ? 2 : 1;
   auto first_block = [&](int item) {
     return item < shares.whole ? item : shares.whole + (item - shares.whole) * shares.spans;
   };
@@ -1041,18 +1056,21 @@ __global__ void __launch_bounds__(kJoinThreads) k_attn_tiles(const AttnArgs a, c
 // ------------------------------------------------------------------ host
 struct Plan {
   int tile_rows, most_spans, blocks, slots;
+  bool alternate;
 };
 Plan plan(const AttnArgs& a, int max_q_len, int max_kv_len) {
   Plan p;
   const int sms = device_sm_count();
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.group;
-  p.tile_rows = static_cast<int64_t>(max_q_len) * a.group <= kRows ? kRows : 2 * kRows;
+  const bool wide = a.kv.head_dim > 128;
+  p.alternate = !wide && static_cast<int64_t>(max_q_len) * a.group <= kRows;
+  p.tile_rows = wide || p.alternate ? kRows : 2 * kRows;
   const int64_t tiles = std::min<int64_t>(rows, rows / p.tile_rows + a.num_seqs);  // a partial one each
   // an item may be cut until a part has 512 keys
   p.most_spans = std::max(1, max_kv_len / 512);
   // whole rounds of items, and a round of parts
   p.blocks = static_cast<int>(tiles * a.kv.kv_heads / sms * sms + sms);
-  p.slots = p.tile_rows == kRows ? 2 * p.blocks : sms;
+  p.slots = p.alternate ? 2 * p.blocks : sms;
   return p;
 }
 size_t round256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -1106,6 +1124,7 @@ struct Many {
     ta.sms = device_sm_count();
     ta.most_spans = p.most_spans;
     ta.tile_rows = p.tile_rows;
+    ta.alternate = p.alternate;
     CUtensorMap maps[2] = {};
     ta.tma = BITS == 16 && cache_map(&maps[0], a.kv, a.kv.k, std::is_same_v<T, __nv_bfloat16>) &&
              cache_map(&maps[1], a.kv, a.kv.v, std::is_same_v<T, __nv_bfloat16>);
@@ -1122,7 +1141,8 @@ template <typename F>
 auto with_many(int bits, bool bf16, int head_dim, F&& f) {
   auto dim = [&](auto t, auto b) {
     if (head_dim <= 64) return f(Many<decltype(t), decltype(b)::value, 64>());
-    return f(Many<decltype(t), decltype(b)::value, 128>());
+    if (head_dim <= 128) return f(Many<decltype(t), decltype(b)::value, 128>());
+    return f(Many<decltype(t), decltype(b)::value, 256>());
   };
   auto form = [&](auto t) {
     if (bits == 16) return dim(t, std::integral_constant<int, 16>());
