@@ -127,8 +127,6 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Shared memory is read by its 32-bit address: the compiler does not see through the
-// aligned base and would read generically.
 // 64 columns x 16 tokens of one page and head (no multicast).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
@@ -136,6 +134,8 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
+// Shared memory is read by its 32-bit address: the compiler does not see through the
+// aligned base and would read generically.
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");

@@ -9,8 +9,8 @@
 // leaves nothing) as the winner of a race, argmax_j w_j / e_j with exponential e_j: that
 // samples from w / sum(w) without its sum, and a maximum does not hang on the order in
 // which the vocabulary is split, as a running sum would. Ties go to the lowest index.
-// A row with a NaN, a +inf or nothing finite, or a temperature that is negative or not finite, has
-// no distribution: its draft is not taken and its token is -1.
+// A row with a NaN, a +inf or nothing finite, or a temperature that is negative or not
+// finite, has no distribution: its draft is not taken and its token is -1.
 //
 // Two launches: every row's maximum and sum over parts of the vocabulary (one pass over
 // the logits, the traffic's bulk), then the decisions and the race over parts of one row
