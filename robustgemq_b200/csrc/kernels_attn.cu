@@ -45,11 +45,6 @@ namespace gemq {
 namespace {
 
 // ------------------------------------------------------------------ small pieces
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }

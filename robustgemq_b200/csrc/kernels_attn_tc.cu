@@ -18,10 +18,12 @@
 // load: 16-bit rows by TMA, codes by way of registers, unpacked to exact fp16 as they are
 // stored.
 //
-// Codes: the steps of values enter as w'_j = w_j t_j / 2^E with one E a block, the
-// largest exponent of a step so far, and o = 2^E sum_j w'_j (d_j + y_j / t_j) / sum_j w_j.
-// A key then has two factors (four at 4 bits) that its 256 rows read from shared memory;
-// the form of kernels_attn.cu has one more, and their delivery is this kernel's bound.
+// Codes: a key's factors (its step and the value's as a shift, 1 / t; at 4 bits also z and
+// y / t) are prepared once by the loaders, and its 256 rows read them from shared memory.
+// The value's step shifts the score, as in kernels_attn.cu, so that a row's reference
+// follows the largest w_j t_j among the keys that it sees: with one exponent for all keys
+// of a block in its place a large step that a row does not see, or gives no weight, pushed
+// its own weights out of fp16's range.
 //
 // The reference of the exponentials moves only when a row's scores pass it by more than
 // 2^8 (in 16 bits 2^8 is as exact as 1), so that the sums in tensor memory are rarely
@@ -34,14 +36,15 @@
 // same 128 rows and all keys, 64 at a time, and half of V's columns each. S and P are formed
 // twice, so two of six products are repeated, but Q and the keys stand in shared memory
 // once, and all else stays as it is. (2,048 tokens at the end of 8,192, 16 query and 4 KV
-// heads x 256: 334 us, 720 TFLOP/s, at 16 bits, where 16-row tiles took 3,141; 819 and 890
+// heads x 256: 334 us, 720 TFLOP/s, at 16 bits, where 16-row tiles took 3,141; 711 and 730
 // at 8 and 4 bits, the loaders' unpacking, against 2,810 and 1,683.)
 //
 // Measured on a B200: 4,096 tokens at the end of 16,384, 32 query and 8 KV heads x 128,
 // bf16: 890 us (1,080 TFLOP/s of the visible pairs; 1,020 us in long runs under the power
 // limit), the exponentials' pipe and the softmax warps' issue. 12 uneven chunks up to 1,000
-// of 9,000, 24 on 8 heads x 64, window 4,096, 8 bits: 489 us (300 TFLOP/s), the factors' reads
-// and the exponentials, which half as many columns leave twice as often.
+// of 9,000, 24 on 8 heads x 64, window 4,096, 8 bits: 480 us (327 TFLOP/s), the softmax
+// warps' chain of waits, factors and exponentials, which half as many columns leave twice as
+// often.
 #define GEMQ_OWN_ERROR_WORDS  // compiled without relocatable device code, for setmaxnreg
 #include <cudaTypedefs.h>
 
@@ -75,9 +78,9 @@ struct Tc {
   static constexpr int kQOff = 0;
   static constexpr int kRingOff = (kWide ? 1 : 2) * kQTile;
   static constexpr int kPrepOff = kRingOff + kStages * kTile;   // per key factors, two tiles
-  static constexpr int kPrepTile = BITS == 16 ? 0 : (BITS == 8 ? 2 : 4) * kKeys * 4;
+  static constexpr int kPrepTile = BITS == 16 ? 0 : (BITS == 8 ? 3 : 5) * kKeys * 4;
   static constexpr int kBarOff = kPrepOff + 2 * kPrepTile;
-  static constexpr int kBars = 2 * kStages + 16;
+  static constexpr int kBars = 2 * kStages + 14;
   static constexpr int kSmem = kBarOff + kBars * 8 + 128 + 1024;  // + alignment
   static_assert(kSmem <= 227 * 1024, "shared memory");
   // Registers after the split: 256 x (184 + 72) = 512 x 128, what the block starts with (a
@@ -253,13 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   uint64_t* const o_done = s_full + 4;          // [2] P V done
   uint64_t* const prep_full = s_full + 6;       // [2]
   uint64_t* const prep_empty = s_full + 8;      // [2]
-  uint64_t* const exp_full = s_full + 10;      // [2] exponents of the steps written
-  uint64_t* const drain = s_full + 12;          // [2]
-  uint64_t* const s_free = s_full + 14;         // [2] S in registers
+  uint64_t* const drain = s_full + 10;          // [2]
+  uint64_t* const s_free = s_full + 12;         // [2] S in registers
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + K::kBars);
   int* const s_odd = reinterpret_cast<int*>(s_tmem + 1);
-  int* const s_exp = s_odd + 1;                 // [2][4] largest step exponent, a loader warp
-  int* const s_e = s_exp + 8;                   // [2] E of the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.kv.head_dim;
   const bool alternate = !K::kWide && ta.alternate, same_rows = K::kWide || alternate;
@@ -346,7 +346,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       mbar_init(&o_done[i], 1);
       mbar_init(&prep_full[i], 4);
       mbar_init(&prep_empty[i], 4 * chains);  // softmax warps
-      mbar_init(&exp_full[i], 4);
       mbar_init(&drain[i], 1);
       mbar_init(&s_free[i], 4);
     }
@@ -594,9 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       }
     } else {
       const bool wide = BITS == 8 || row_bytes % 16 == 0;
-      int exp_now = -126;  // E
-      // Steps of the tile's keys, one a loader, two tiles ahead: of the tile after the one
-      // whose codes are being asked for the loaders exchange the largest exponent.
+      // Steps of the tile's keys, one a loader, asked for a tile ahead.
       float2 ksc = make_float2(0.f, 0.f), vsc = ksc;
       auto ask_steps = [&](int t) {
         ksc = vsc = make_float2(0.f, 0.f);
@@ -612,11 +609,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           ksc = __ldg(reinterpret_cast<const float2*>(a.kv.k_scale + at));
           vsc = __ldg(reinterpret_cast<const float2*>(a.kv.v_scale + at));
         }
-      };
-      auto tell_exponent = [&](int t) {
-        const int e = __reduce_max_sync(0xffffffffu, vsc.x < INFINITY ? ilogbf(fmaxf(vsc.x, kMinScale)) : -126);
-        if (lane == 0) s_exp[(t & 1) * 4 + (me >> 5)] = e;
-        warp_arrive(&exp_full[t & 1]);
       };
       auto fetch_codes = [&](const Rows& x, int t, const uint8_t* base, uint4 (&raw)[kIts]) {
         if (x.live[0] == kIts && wide) {  // all in one page, as nearly always
@@ -675,27 +667,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         warp_arrive(&full[g % kStages]);
       };
       auto factors = [&](int t, float2 kstep, float2 vstep) {
-        ok = warp_wait(&prep_empty[t & 1], ((t >> 1) & 1) ^ 1u, kDevTimeoutAEmpty) &&
-             warp_wait(&exp_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
+        ok = warp_wait(&prep_empty[t & 1], ((t >> 1) & 1) ^ 1u, kDevTimeoutAEmpty);
         if (!ok) return;
-        // the key's factors: a = s c, t / 2^E (and z c, y / t), with c = scale log2(e). A
-        // poisoned step of either makes a NaN in a, which reaches the weights of the rows
+        // the key's factors: a = s c, log2 t, 1 / t (and z c, y / t), with c = scale log2(e).
+        // A poisoned step of either makes a NaN in a, which reaches the weights of the rows
         // that see the key and no others; the rest must then be numbers.
-#pragma unroll
-        for (int w = 0; w < 4; ++w) exp_now = max(exp_now, s_exp[(t & 1) * 4 + w]);
         if (me < kKeys) {
           float* const prep = s_prep + (t & 1) * (K::kPrepTile / 4);
           const float vs = vstep.x < kMinScale ? kMinScale : vstep.x;  // a step of zero; a NaN stays
+          const float lv = lg2(vs);
           bool bad = !(vs < INFINITY);
           if constexpr (BITS == 4) {
             const float zr = fmaf(8.f, vstep.x, vstep.y) / vs;
             bad = bad || !(fabsf(zr) < INFINITY);
-            prep[2 * kKeys + me] = fmaf(8.f, kstep.x, kstep.y) * cs;
-            prep[3 * kKeys + me] = bad ? 0.f : zr;
+            prep[3 * kKeys + me] = fmaf(8.f, kstep.x, kstep.y) * cs;
+            prep[4 * kKeys + me] = bad ? 0.f : zr;
           }
           prep[me] = bad ? NAN : kstep.x * cs;
-          prep[kKeys + me] = bad ? 0.f : vs * exp2f(static_cast<float>(-exp_now));
-          if (me == 0) s_e[t & 1] = exp_now;
+          prep[kKeys + me] = bad ? 0.f : lv;
+          prep[2 * kKeys + me] = bad ? 0.f : ex2(-lv);
         }
         warp_arrive(&prep_full[t & 1]);
       };
@@ -707,7 +697,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       ask_pages(1);
       if (n_tiles > 0) {
         fetch_codes(x, 0, a.kv.k, raw_k);
-        tell_exponent(0);
       }
       for (int t = 0; t < n_tiles && ok; ++t) {
         fetch_codes(x, t, a.kv.v, raw_v);
@@ -720,7 +709,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           x = rows_of(t + 1);
           ask_pages(t + 2);
           fetch_codes(x, t + 1, a.kv.k, raw_k);
-          tell_exponent(t + 1);
         }
         store_codes(2 * t + 1, raw_v);
       }
@@ -792,7 +780,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     const int w_max = pos0 + (row0 + min(w_row + 31, max(rows, 1) - 1)) / a.group;
     const int cols = K::num_cols(chain, D);
     float ref = -INFINITY, l = 0.f, zacc = 0.f;
-    int e_now = -126;  // E of the sums so far
     int n = 0;
     for (int t = chain_first(chain); t < n_tiles && ok; t += step, ++n) {
       const int j0 = (k0 + t) * kKeys;
@@ -811,20 +798,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       warp_arrive(&s_free[chain]);
       auto sf = [&](int j) { return __uint_as_float(s[j]); };
       if constexpr (BITS != 16) {
-        // scores of codes
+        // scores of codes, the value's step as a shift
         const F2 qs2 = f2(qsum, qsum), rf2 = f2(rf, rf);
 #pragma unroll
         for (int j = 0; j < kKeys; j += 4) {
-          F2 a2[2], z2[2];
+          F2 a2[2], lv2[2], z2[2];
           lds_pairs(prep + 4 * j, a2);
-          if constexpr (BITS == 4) lds_pairs(prep + 4 * (2 * kKeys + j), z2);
+          lds_pairs(prep + 4 * (kKeys + j), lv2);
+          if constexpr (BITS == 4) lds_pairs(prep + 4 * (3 * kKeys + j), z2);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const F2 s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
             F2 x;
-            if constexpr (BITS == 4) x = fma2(s2, a2[e], mul2(qs2, z2[e]));
-            else x = mul2(s2, a2[e]);
-            if constexpr (K::kRowFactor) x = mul2(x, rf2);
+            if constexpr (K::kRowFactor) {
+              x = mul2(s2, a2[e]);
+              if constexpr (BITS == 4) x = fma2(qs2, z2[e], x);
+              x = fma2(x, rf2, lv2[e]);
+            } else {
+              if constexpr (BITS == 4) lv2[e] = fma2(qs2, z2[e], lv2[e]);
+              x = fma2(s2, a2[e], lv2[e]);
+            }
             float x0, x1;
             split(x, x0, x1);
             s[j + 2 * e] = __float_as_uint(x0);
@@ -846,18 +839,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * (BITS == 16 ? cs : 1.f);
       // a row whose reference is not set yet, or is left behind, takes its maximum
       const bool behind = ref == -INFINITY ? top > -INFINITY : top > ref + kSlack;
-      int e_tile = e_now;
-      if constexpr (BITS != 16) e_tile = s_e[t & 1];
-      if (__any_sync(0xffffffffu, behind || e_tile != e_now)) {
+      if (__any_sync(0xffffffffu, behind)) {
         const float now = behind ? top : ref;
-        float keep = now == -INFINITY ? 1.f : ex2(ref - now);  // ref = -inf: 0
+        const float keep = now == -INFINITY ? 1.f : ex2(ref - now);  // ref = -inf: 0
         l *= keep;
+        zacc *= keep;
         ref = now;
-        if constexpr (BITS != 16) {
-          keep *= ex2(static_cast<float>(max(e_now - e_tile, -126)));
-          zacc *= keep;
-          e_now = e_tile;
-        }
         if (n > 0) {
           ok = warp_wait(&o_done[chain], (n - 1) & 1, kDevTimeoutAccFull);
           if (!ok) break;
@@ -881,19 +868,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
 #pragma unroll
         for (int i = from_i; i < to_i; i += 2) {
           const int j = 2 * i;
-          F2 tv[2], zr[2];
-          if constexpr (BITS != 16) lds_pairs(prep + 4 * (kKeys + j), tv);
-          if constexpr (BITS == 4) lds_pairs(prep + 4 * (3 * kKeys + j), zr);
+          F2 inv[2], zr[2];
+          if constexpr (BITS != 16) lds_pairs(prep + 4 * (2 * kKeys + j), inv);
+          if constexpr (BITS == 4) lds_pairs(prep + 4 * (4 * kKeys + j), zr);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const F2 s2 = f2(sf(j + 2 * e), sf(j + 2 * e + 1));
             float y0, y1;
             split(BITS == 16 ? fma2(s2, cs2, base2) : add2(s2, base2), y0, y1);
-            F2 w = f2(ex2(y0), ex2(y1));
-            lt[e] = add2(lt[e], w);
-            if constexpr (BITS != 16) w = mul2(w, tv[e]);
-            float w0, w1;
-            split(w, w0, w1);
+            const float w0 = ex2(y0), w1 = ex2(y1);
+            const F2 w = f2(w0, w1);
+            if constexpr (BITS == 16) lt[e] = add2(lt[e], w);
+            else lt[e] = fma2(w, inv[e], lt[e]);
             p[i + e] = pack2<C>(w0, w1);
             if constexpr (BITS == 4) {
               // the rounded weights, so that their rounding scales with the value and not
@@ -937,7 +923,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       const bool in = my_row < rows;
       const int tok = (row0 + my_row) / a.group, hh = (row0 + my_row) % a.group;
       const int64_t at = static_cast<int64_t>(r.start + tok) * a.q_heads + h * a.group + hh;
-      const float up = BITS == 16 ? 1.f : exp2f(static_cast<float>(e_now));  // 2^E
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       const bool cut = ta.cut(shares, block);
       const int64_t slot = cut ? static_cast<int64_t>(ta.slot(shares, block) + (alternate ? chain : 0)) * ta.tile_rows + my_row : 0;
@@ -955,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
           for (int e = 0; e < 16; ++e) {
             // a 4-bit row's columns stand in the order its codes unpack
             const int d = BITS == 4 ? (e & 8) + place4(e & 7) : e;
-            x[d] = BITS == 16 ? __uint_as_float(o[e]) : (__uint_as_float(o[e]) + zacc) * up;
+            x[d] = BITS == 16 ? __uint_as_float(o[e]) : __uint_as_float(o[e]) + zacc;
           }
         } else {
 #pragma unroll
