@@ -217,6 +217,7 @@ struct TileArgs {
   float* o;        // [slots][tile rows][DP]: parts of rows
   float2* ml;      // [slots][tile rows]
   int sms;
+  int most_tiles;  // row tiles that the grid and the buffers are planned for
   int most_spans;  // of an item
   int tile_rows;   // 256; 128 where both chains take the same rows
   bool alternate;  // they take every second tile of keys each
@@ -274,10 +275,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   // Tiles in descending order of their position: of a causal sequence's tiles the last
   // ones are the longest, and the short ones fill the machine's end.
   auto tiles_of = [&](int b) { return (seq_range(a, b).q_len * a.group + ta.tile_rows - 1) / ta.tile_rows; };
-  int total = 0;
-  for (int b = lane; b < a.num_seqs; b += 32) total += tiles_of(b);
+  int64_t tiles = 0;
+  for (int b = lane; b < a.num_seqs; b += 32) tiles += tiles_of(b);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+  // Starts that go back give several sequences the same tokens, and more tiles than the
+  // call's tokens have: those past the plan are left out.
+  if (tiles > ta.most_tiles) set_device_error(kDevBadCachePos);
+  const int total = static_cast<int>(min(tiles, static_cast<int64_t>(ta.most_tiles)));
   const int block = static_cast<int>(blockIdx.x);
   const Shares shares = ta.share(total * a.kv.kv_heads);
   if (block == 0 && threadIdx.x == 0) *ta.shares = shares;
@@ -1040,7 +1045,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attn_tiles(const AttnArgs a, c
 
 // ------------------------------------------------------------------ host
 struct Plan {
-  int tile_rows, most_spans, blocks, slots;
+  int tile_rows, tiles, most_spans, blocks, slots;
   bool alternate;
 };
 Plan plan(const AttnArgs& a, int max_q_len, int max_kv_len) {
@@ -1050,11 +1055,11 @@ Plan plan(const AttnArgs& a, int max_q_len, int max_kv_len) {
   const bool wide = a.kv.head_dim > 128;
   p.alternate = !wide && static_cast<int64_t>(max_q_len) * a.group <= kRows;
   p.tile_rows = wide || p.alternate ? kRows : 2 * kRows;
-  const int64_t tiles = std::min<int64_t>(rows, rows / p.tile_rows + a.num_seqs);  // a partial one each
+  p.tiles = static_cast<int>(std::min<int64_t>(rows, rows / p.tile_rows + a.num_seqs));  // a partial one each
   // an item may be cut until a part has 512 keys
   p.most_spans = std::max(1, max_kv_len / 512);
   // whole rounds of items, and a round of parts
-  p.blocks = static_cast<int>(tiles * a.kv.kv_heads / sms * sms + sms);
+  p.blocks = static_cast<int>(static_cast<int64_t>(p.tiles) * a.kv.kv_heads / sms * sms + sms);
   p.slots = p.alternate ? 2 * p.blocks : sms;
   return p;
 }
@@ -1107,6 +1112,7 @@ struct Many {
     ta.o = reinterpret_cast<float*>(w);
     ta.ml = reinterpret_cast<float2*>(ta.o + static_cast<size_t>(p.slots) * p.tile_rows * DP);
     ta.sms = device_sm_count();
+    ta.most_tiles = p.tiles;
     ta.most_spans = p.most_spans;
     ta.tile_rows = p.tile_rows;
     ta.alternate = p.alternate;
