@@ -67,7 +67,7 @@ __device__ void attn_one_row(const AttnArgs& a, int b, const SeqRange& r, int i,
   __syncthreads();
   const int pos = r.kv_len - r.q_len + i;
   const int j1 = min(pos, r.kv_len - 1) + 1;
-  const int j0 = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  const int j0 = first_seen(pos, a.window);
   const int mask = (1 << a.kv.page_shift) - 1;
   float m = -INFINITY, l = 0.f, o[kAttnMaxDim / kAttnRowThreads] = {};
   for (int jb = j0; jb < j1; jb += kAttnRowThreads) {

@@ -170,8 +170,7 @@ __device__ __forceinline__ SeqPlan plan_seq(const AttnArgs& a, int b, int unit) 
   SeqPlan p;
   p.r = seq_range(a, b);
   p.row_tiles = (p.r.q_len * a.group + M - 1) / M;
-  const int lo = a.window > 0 ? max(0, p.r.kv_len - p.r.q_len - a.window + 1) : 0;
-  p.t0 = lo / unit;
+  p.t0 = first_seen(p.r.kv_len - p.r.q_len, a.window) / unit;
   p.units = max(1, (p.r.kv_len + unit - 1) / unit - p.t0);
   return p;
 }
@@ -489,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, BITS, DP, NR>::kBlocks) k_att
       for (int e = 0; e < 2; ++e) {
         const int c = 8 * i + 2 * tig + e;
         last[i][e] = c < rows ? pos0 + (rt * kM + c) / a.group : -1;
-        from[i][e] = a.window > 0 ? max(0, last[i][e] - a.window + 1) : 0;
+        from[i][e] = first_seen(last[i][e], a.window);
         if constexpr (BITS != 16) {
           rf[i][e] = __shfl_sync(0xffffffffu, factor, (2 * tig + e) * 4);
           qsum[i][e] = __shfl_sync(0xffffffffu, sum, (2 * tig + e) * 4);
@@ -634,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, BITS, DP, NR>::kBlocks) k_att
               }
           }
       }
-      const bool full = j0 + kKeys - 1 <= tile_min && (a.window <= 0 || j0 > tile_max - a.window);
+      const bool full = j0 + kKeys - 1 <= tile_min && (a.window <= 0 || tile_max - j0 < a.window);
       if (!full) {
 #pragma unroll
         for (int i = 0; i < kMt; ++i)
@@ -654,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, BITS, DP, NR>::kBlocks) k_att
               const bool odd = !(inv[i][hi] < INFINITY) || (BITS == 4 && !(fabsf(zr[i][hi]) < INFINITY));
               const int j = j0 + 16 * i + 8 * hi + gid;
               if (odd && j > tile_min) inv[i][hi] = zr[i][hi] = 0.f;
-              if (odd && a.window > 0 && j <= tile_max - a.window) inv[i][hi] = zr[i][hi] = 0.f;
+              if (odd && a.window > 0 && tile_max - j >= a.window) inv[i][hi] = zr[i][hi] = 0.f;
             }
         }
       }

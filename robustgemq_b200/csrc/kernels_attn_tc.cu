@@ -324,8 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
   // key tiles [k0, k1) of this span, the first key of key tile 0 is 0
   int k0 = 0, k1 = 0;
   if (work) {
-    const int lo = a.window > 0 ? max(0, tile_min - a.window + 1) : 0;
-    const int t0 = lo / kKeys, n = max(0, (tile_max + 1 + kKeys - 1) / kKeys - t0);
+    const int t0 = first_seen(tile_min, a.window) / kKeys, n = max(0, (tile_max + 1 + kKeys - 1) / kKeys - t0);
     k0 = t0 + static_cast<int>(static_cast<int64_t>(n) * span / spans);
     k1 = t0 + static_cast<int>(static_cast<int64_t>(n) * (span + 1) / spans);
   }
@@ -372,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     const int tok = (row0 + my_row) / a.group, hh = (row0 + my_row) % a.group;
     if (in) {
       last = pos0 + tok;
-      from = a.window > 0 ? max(0, last - a.window + 1) : 0;
+      from = first_seen(last, a.window);
     }
     const T* q = static_cast<const T*>(a.q) +
                  (in ? (r.start + tok) * a.q_token_stride + static_cast<int64_t>(h * a.group + hh) * D : 0);
@@ -524,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
       int armed = 0;  // stages filled so far
       for (int t = 0; t < n_tiles && ok; ++t) {
         const int j0 = (k0 + t) * kKeys;
-        const bool mixed = j0 + kKeys - 1 > tile_min || (a.window > 0 && j0 <= tile_max - a.window);
+        const bool mixed = j0 + kKeys - 1 > tile_min || (a.window > 0 && tile_max - j0 >= a.window);
         if (!mixed && ta.tma) {  // (no row sees past the sequence: the tile is inside it)
           int ids[2];
 #pragma unroll
@@ -788,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
     int n = 0;
     for (int t = chain_first(chain); t < n_tiles && ok; t += step, ++n) {
       const int j0 = (k0 + t) * kKeys;
-      const bool whole = j0 + kKeys - 1 <= w_min && (a.window <= 0 || j0 > w_max - a.window);
+      const bool whole = j0 + kKeys - 1 <= w_min && (a.window <= 0 || w_max - j0 < a.window);
       const uint32_t prep = smem_u32(s_prep + (t & 1) * (K::kPrepTile / 4));
       if constexpr (BITS != 16) ok = warp_wait(&prep_full[t & 1], (t >> 1) & 1, kDevTimeoutAFull);
       ok = ok && warp_wait(&s_full[chain], n & 1, kDevTimeoutAccFull);

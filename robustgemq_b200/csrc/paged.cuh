@@ -170,6 +170,12 @@ __device__ __forceinline__ SeqRange seq_range(const AttnArgs& a, int b) {
   return r;
 }
 
+// The first position that a row at position `last` sees. (Neither of the two may be taken
+// from the other as they are: a row before position 0 with the widest window leaves 32 bits.)
+__device__ __forceinline__ int first_seen(int last, int window) {
+  return window > 0 && last >= window ? last - window + 1 : 0;
+}
+
 // The page of a sequence's page index, or -1 (recorded) for an id outside the cache.
 __device__ __forceinline__ int page_of(const AttnArgs& a, int b, int index) {
   const int p = a.page_table[b * a.page_table_stride + index];

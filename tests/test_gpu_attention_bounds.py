@@ -86,3 +86,17 @@ def test_lengths_outside_the_table(lens, max_q_len):
     lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
     guarded_call(b, b.q_starts, lens, b.page_table, max_q_len)
     assert _lib.device_error() == BAD_POSITION
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("n,length", [(1, 70), (6, 3), (6, 700), (200, 70), (200, 1), (300, 700)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_the_widest_windows_hide_nothing(bits, n, length, dim):
+    """2^31 - 1 as "no limit", also with more new tokens than positions."""
+    from robustgemq_b200.serving import paged_attention
+
+    b = Batch([(n, length), (2, 50)], 4, 2, dim, 16, bits, H16)
+    want, _ = b.check()
+    for window in ((1 << 31) - 1, (1 << 31) - 2, max(n, length, 50)):
+        got = paged_attention(b.q, b.cache, b.page_table, b.kv_lens, q_starts=b.q_starts, window=window)
+        assert torch.equal(got, want)
