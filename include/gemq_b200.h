@@ -408,7 +408,8 @@ int gemq_kv_cache_read(const gemq_kv_cache_t* cache /* host */, const int64_t* s
  * q_heads] or NULL: the natural logarithm of the sum of exp(scale * score). Scores,
  * softmax statistics and sums are fp32. Tokens outside every sequence are not written.
  * max_q_len and max_kv_len (0: unknown) are the longest values the call may meet; they
- * choose the kernel and the split, and longer ones stay right. Lengths, starts and page
+ * choose the kernel and the split, and longer ones stay right. A sequence has at most
+ * 2^31 - 1024 positions. Lengths, starts and page
  * ids outside the buffers are clamped or skipped and recorded in the device error word. */
 size_t gemq_paged_attention_workspace_size(const gemq_kv_cache_t* cache /* host */, int64_t num_tokens,
                                            int32_t q_heads, int32_t num_seqs, int32_t max_pages, int32_t max_q_len,

@@ -128,6 +128,10 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+// Positions of a sequence that attention takes: below 2^31 by more than a kernel's tiles and
+// units of keys, and the tiles asked for ahead, reach past the last one.
+constexpr int kMaxPositions = 0x7fffffff - 1023;
+
 // Everything an attention launch needs.
 struct AttnArgs {
   KvDev kv;
@@ -162,7 +166,7 @@ __device__ __forceinline__ SeqRange seq_range(const AttnArgs& a, int b) {
     hi = lo + n;
   }
   const int kv = a.kv_lens[b];
-  const int cap = a.max_pages << a.kv.page_shift;
+  const int cap = min(a.max_pages << a.kv.page_shift, kMaxPositions);
   r.start = min(max(lo, 0), a.num_tokens);
   r.q_len = min(max(hi, r.start), a.num_tokens) - r.start;
   r.kv_len = min(max(kv, 0), cap);

@@ -100,3 +100,25 @@ def test_the_widest_windows_hide_nothing(bits, n, length, dim):
     for window in ((1 << 31) - 1, (1 << 31) - 2, max(n, length, 50)):
         got = paged_attention(b.q, b.cache, b.page_table, b.kv_lens, q_starts=b.q_starts, window=window)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_as_many_positions_as_32_bits_take(n):
+    """2^31 - 1024 positions on one page again and again, all of one weight; longer lengths
+    are clamped to that and recorded. Sums in fp32 of up to 2^21 terms each, rounded or
+    truncated: a quarter at most."""
+    from robustgemq_b200 import _lib
+    from robustgemq_b200.serving import PagedKVCache, paged_attention
+
+    cache = PagedKVCache(1, 16, 1, 16)
+    v = torch.arange(1, 17, device="cuda").half().expand(16, 1, 16).contiguous()
+    cache.write(torch.zeros_like(v), v, torch.arange(16, device="cuda"))
+    table = torch.zeros((1, (1 << 27) - 1), dtype=torch.int32, device="cuda")
+    q = torch.randn((n, 1, 16), device="cuda").half()
+    most = (1 << 31) - 1024
+    for length, code in ((most, 0), (most + 1008, BAD_POSITION)):
+        lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+        out, lse = paged_attention(q, cache, table, lens, return_lse=True)
+        assert _lib.device_error() == code
+        assert ((out.float() / v[0].float() - 1).abs() <= 0.25).all()
+        assert ((lse - 21.4876).abs() <= 0.25).all()  # ln(2^31)
