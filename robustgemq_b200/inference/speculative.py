@@ -15,6 +15,7 @@ time from a static fp16 cache and has no counterpart.
 
 from __future__ import annotations
 
+import math
 from typing import List, Optional, Sequence
 
 import torch
@@ -37,6 +38,13 @@ def lookup_draft(tokens: Sequence[int], most: int, longest: int = 3) -> List[int
     return []
 
 
+def _drawn(token: int) -> int:
+    """The token that the verification drew, where it drew one."""
+    if token < 0:
+        raise RuntimeError("a row of logits has no distribution (a NaN, a +inf or nothing finite)")
+    return token
+
+
 class PagedDecoder:
     """Sequences of one model on paged caches, one a layer, that share a page table."""
 
@@ -53,6 +61,7 @@ class PagedDecoder:
         self.kv_heads = model.config.num_key_value_heads
         if self.kv_heads != self.heads:
             raise ValueError("the fused query, key and value projection has as many KV heads as heads")
+        self.vocab = model.model.embed_tokens.weight.shape[0]
         self.page_size = page_size
         self.caches = [PagedKVCache(num_pages, page_size, self.kv_heads, self.head_dim, bits=bits,
                                     dtype=torch.float16, device=self.device) for _ in layers]
@@ -90,6 +99,8 @@ class PagedDecoder:
         counts = [len(c) for c in chunks]
         if not counts or min(counts) < 1 or len(counts) != len(seqs):
             raise ValueError("one chunk of at least one token a sequence")
+        if not all(0 <= t < self.vocab for c in chunks for t in c):
+            raise ValueError(f"a token outside the vocabulary of {self.vocab}")
         lens = [self.lengths[s] + n for s, n in zip(seqs, counts)]
         for s, n in zip(seqs, lens):
             self._reserve(s, n)
@@ -143,7 +154,10 @@ class PagedDecoder:
                  temperature: float = 0.0, chunk: int = 512, generator: Optional[torch.Generator] = None):
         """Continues every prompt by ``max_new_tokens`` tokens, greedily or sampled at
         ``temperature``, with up to ``drafts`` looked-up tokens a step. Returns the new
-        tokens of each prompt and ``{"steps", "drafted", "accepted"}``."""
+        tokens of each prompt and ``{"steps", "drafted", "accepted"}``. A row of logits without
+        a distribution (a NaN, a +inf, nothing finite) is an error."""
+        if not (0 <= temperature < math.inf):
+            raise ValueError("temperature must be finite and not negative")
         seqs = [self.add_sequence() for _ in prompts]
         tokens = [list(p) for p in prompts]
         dev = self.device
@@ -164,7 +178,7 @@ class PagedDecoder:
         first = verify_draft(torch.stack(last)[:, None].expand(-1, 2, -1).contiguous(), none[:, None].long(),
                              torch.zeros((len(seqs), 1), device=dev), noise(len(seqs)), draft_lens=none, temperature=temps)
         for i, t in enumerate(first.tokens[:, 0].tolist()):
-            tokens[i].append(t)
+            tokens[i].append(_drawn(t))
         stats = {"steps": 0, "drafted": 0, "accepted": 0}
         done = [len(p) + max_new_tokens for p in prompts]
         while True:
@@ -178,7 +192,7 @@ class PagedDecoder:
             taken = r.num_accepted.tolist()
             out = r.tokens.tolist()
             for i, g, a, row in zip(live, guess, taken, out):
-                tokens[i] += row[:a + 1]
+                tokens[i] += row[:a] + [_drawn(row[a])]
                 self.advance(seqs[i], a + 1)
                 stats["drafted"] += len(g)
                 stats["accepted"] += a
