@@ -158,7 +158,16 @@ class PagedDecoder:
         a distribution (a NaN, a +inf, nothing finite) is an error."""
         if not (0 <= temperature < math.inf):
             raise ValueError("temperature must be finite and not negative")
-        seqs = [self.add_sequence() for _ in prompts]
+        seqs: List[int] = []
+        try:
+            for _ in prompts:
+                seqs.append(self.add_sequence())
+            return self._continue(seqs, prompts, max_new_tokens, drafts, float(temperature), chunk, generator)
+        finally:
+            for s in seqs:
+                self.release(s)
+
+    def _continue(self, seqs, prompts, max_new_tokens, drafts, temperature, chunk, generator):
         tokens = [list(p) for p in prompts]
         dev = self.device
         last: List[Optional[Tensor]] = [None] * len(seqs)
@@ -172,7 +181,7 @@ class PagedDecoder:
         def noise(n):
             return torch.empty((n, vocab), device=dev).exponential_(generator=generator)
 
-        temps = torch.full((len(seqs),), float(temperature), device=dev)
+        temps = torch.full((len(seqs),), temperature, device=dev)
         # the first token: one draft that counts for nothing, so that the race decides
         none = torch.zeros((len(seqs),), dtype=torch.int32, device=dev)
         first = verify_draft(torch.stack(last)[:, None].expand(-1, 2, -1).contiguous(), none[:, None].long(),
@@ -197,8 +206,6 @@ class PagedDecoder:
                 stats["drafted"] += len(g)
                 stats["accepted"] += a
             stats["steps"] += 1
-        for s in seqs:
-            self.release(s)
         return [t[len(p):] for t, p in zip(tokens, prompts)], stats
 
     def _verify(self, logits, guess, width, temps, noise, generator) -> Verified:

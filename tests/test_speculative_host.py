@@ -94,3 +94,25 @@ def test_tokens_outside_the_vocabulary_do_not_reach_the_model(decoder, monkeypat
     with pytest.raises(ValueError, match="vocabulary"):
         decoder.forward([s], [[1, token, 2]])
     assert decoder.pages[s] == []
+
+
+def test_pages_come_back_after_an_error(decoder):
+    with pytest.raises(RuntimeError, match="full"):
+        decoder.generate([[1] * 12, [2] * 12, [3] * 12], 4)
+    assert sorted(decoder.free) == list(range(8))
+    new, _ = decoder.generate([[1, 2, 3]], 3)
+    assert new == [[4, 5, 6]]
+
+
+def test_pages_come_back_after_a_step_that_failed(decoder, monkeypatch):
+    whole = decoder.forward
+
+    def run(seqs, chunks):
+        if len(decoder.seen) == 3:
+            raise KeyError("no")
+        return whole(seqs, chunks)
+
+    monkeypatch.setattr(decoder, "forward", run)
+    with pytest.raises(KeyError):
+        decoder.generate([[1, 2], [3]], 5)
+    assert sorted(decoder.free) == list(range(8)) and decoder.lengths == [0, 0]
