@@ -69,10 +69,13 @@ class PagedDecoder:
         self.width = max_pages_per_seq or num_pages
         self.pages: List[List[int]] = []   # of each sequence
         self.lengths: List[int] = []       # positions in the cache
+        self.idle: List[int] = []          # released numbers, to be given out again
         self.page_table = torch.zeros((0, self.width), dtype=torch.int32, device=self.device)
 
     def add_sequence(self) -> int:
-        """A new empty sequence; returns its number."""
+        """A new empty sequence; returns its number (a released one, where there is one)."""
+        if self.idle:
+            return self.idle.pop()
         self.pages.append([])
         self.lengths.append(0)
         row = torch.zeros((1, self.width), dtype=torch.int32, device=self.device)
@@ -101,6 +104,7 @@ class PagedDecoder:
             raise ValueError("one chunk of at least one token a sequence")
         if not all(0 <= t < self.vocab for c in chunks for t in c):
             raise ValueError(f"a token outside the vocabulary of {self.vocab}")
+        self.idle = [s for s in self.idle if s not in seqs]  # (a released sequence, begun anew)
         lens = [self.lengths[s] + n for s, n in zip(seqs, counts)]
         for s, n in zip(seqs, lens):
             self._reserve(s, n)
@@ -144,10 +148,12 @@ class PagedDecoder:
         self.lengths[seq] += tokens
 
     def release(self, seq: int) -> None:
-        """Gives a sequence's pages back."""
+        """Gives a sequence's pages back, and its number to the next new sequence."""
         self.free += reversed(self.pages[seq])
         self.pages[seq] = []
         self.lengths[seq] = 0
+        if seq not in self.idle:
+            self.idle.append(seq)
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, drafts: int = 4,

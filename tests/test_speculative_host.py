@@ -116,3 +116,16 @@ def test_pages_come_back_after_a_step_that_failed(decoder, monkeypatch):
     with pytest.raises(KeyError):
         decoder.generate([[1, 2], [3]], 5)
     assert sorted(decoder.free) == list(range(8)) and decoder.lengths == [0, 0]
+
+
+def test_released_numbers_are_given_out_again(decoder):
+    """Many calls on one decoder do not grow its tables."""
+    for _ in range(5):
+        decoder.generate([[1, 2], [3], [4]], 3)
+    assert decoder.page_table.shape[0] == len(decoder.pages) == len(decoder.lengths) == 3
+    a = decoder.add_sequence()
+    b = decoder.add_sequence()
+    decoder.release(a)
+    decoder.release(a)
+    c, d = decoder.add_sequence(), decoder.add_sequence()
+    assert c == a and len({b, c, d}) == 3
