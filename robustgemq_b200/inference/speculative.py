@@ -164,6 +164,12 @@ class PagedDecoder:
         a distribution (a NaN, a +inf, nothing finite) is an error."""
         if not (0 <= temperature < math.inf):
             raise ValueError("temperature must be finite and not negative")
+        if max_new_tokens < 0 or drafts < 0 or chunk < 1:
+            raise ValueError("max_new_tokens and drafts must not be negative, chunk must be positive")
+        if not all(len(p) for p in prompts):
+            raise ValueError("a prompt needs at least one token")
+        if len(prompts) == 0 or max_new_tokens == 0:
+            return [[] for _ in prompts], {"steps": 0, "drafted": 0, "accepted": 0}
         seqs: List[int] = []
         try:
             for _ in prompts:

@@ -129,3 +129,20 @@ def test_released_numbers_are_given_out_again(decoder):
     decoder.release(a)
     c, d = decoder.add_sequence(), decoder.add_sequence()
     assert c == a and len({b, c, d}) == 3
+
+
+def test_nothing_to_generate(decoder):
+    none = {"steps": 0, "drafted": 0, "accepted": 0}
+    assert decoder.generate([[1, 2], [3]], 0) == ([[], []], none)
+    assert decoder.generate([], 5) == ([], none)
+    assert decoder.seen == [] and decoder.generate([[1]], 1)[0] == [[2]]
+
+
+@pytest.mark.parametrize("args,text", [
+    (dict(prompts=[[1], []]), "prompt"), (dict(max_new_tokens=-1), "max_new_tokens"), (dict(drafts=-1), "drafts"),
+    (dict(chunk=0), "chunk"),
+])
+def test_generate_refusals(decoder, args, text):
+    with pytest.raises(ValueError, match=text):
+        decoder.generate(**(dict(prompts=[[1, 2]], max_new_tokens=3) | args))
+    assert decoder.seen == [] and sorted(decoder.free) == list(range(8))
