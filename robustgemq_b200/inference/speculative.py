@@ -102,6 +102,8 @@ class PagedDecoder:
         counts = [len(c) for c in chunks]
         if not counts or min(counts) < 1 or len(counts) != len(seqs):
             raise ValueError("one chunk of at least one token a sequence")
+        if len(set(seqs)) != len(seqs) or not all(0 <= s < len(self.pages) for s in seqs):
+            raise ValueError("sequences must be numbers of add_sequence, each once a call")
         if not all(0 <= t < self.vocab for c in chunks for t in c):
             raise ValueError(f"a token outside the vocabulary of {self.vocab}")
         self.idle = [s for s in self.idle if s not in seqs]  # (a released sequence, begun anew)

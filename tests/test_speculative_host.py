@@ -146,3 +146,13 @@ def test_generate_refusals(decoder, args, text):
     with pytest.raises(ValueError, match=text):
         decoder.generate(**(dict(prompts=[[1, 2]], max_new_tokens=3) | args))
     assert decoder.seen == [] and sorted(decoder.free) == list(range(8))
+
+
+@pytest.mark.parametrize("seqs", [[0, 0], [0, 2], [-1, 0]])
+def test_forward_takes_a_sequence_once(decoder, monkeypatch, seqs):
+    """Two chunks of one sequence would be written to the same places."""
+    monkeypatch.undo()
+    decoder.add_sequence(), decoder.add_sequence()
+    with pytest.raises(ValueError, match="once a call"):
+        decoder.forward(seqs, [[1, 2], [3]])
+    assert decoder.pages == [[], []]
