@@ -408,7 +408,9 @@ int gemq_kv_cache_read(const gemq_kv_cache_t* cache /* host */, const int64_t* s
  * q_heads] or NULL: the natural logarithm of the sum of exp(scale * score). Scores,
  * softmax statistics and sums are fp32. Tokens outside every sequence are not written.
  * max_q_len and max_kv_len (0: unknown) are the longest values the call may meet; they
- * choose the kernel and the split, and longer ones stay right. A sequence has at most
+ * choose the kernel and the split, and longer ones stay right. An unknown max_q_len is
+ * taken for num_tokens, so give it where many sequences have a few tokens each, also
+ * without q_starts (num_tokens / num_seqs). A sequence has at most
  * 2^31 - 1024 positions. Lengths, starts and page
  * ids outside the buffers are clamped or skipped and recorded in the device error word. */
 size_t gemq_paged_attention_workspace_size(const gemq_kv_cache_t* cache /* host */, int64_t num_tokens,

@@ -4,6 +4,8 @@
 // step took 17 us to issue, of which its two launches are 6).
 #include <torch/extension.h>
 
+#include <algorithm>
+
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -148,6 +150,8 @@ std::pair<Tensor, OptTensor> attention(Tensor q, const Cache& cache, Tensor page
   Tensor out = at::empty({tokens, heads, q.size(2)}, q.options());
   OptTensor lse;
   if (return_lse) lse = at::empty({tokens, heads}, q.options().dtype(at::kFloat));
+  // without starts every sequence's tokens are as many as there are for it
+  if (!q_starts && seqs > 0) max_q_len = std::min<int64_t>(tokens / seqs, INT32_MAX);
   const auto h = static_cast<int32_t>(heads), s = static_cast<int32_t>(seqs), p = static_cast<int32_t>(pages),
              mq = static_cast<int32_t>(max_q_len), mk = static_cast<int32_t>(max_kv_len);
   const size_t need = gemq_paged_attention_workspace_size(&cache.c, tokens, h, s, p, mq, mk);

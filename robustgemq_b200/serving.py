@@ -97,8 +97,11 @@ def paged_attention(q: Tensor, cache: PagedKVCache, page_table: Tensor, kv_lens:
     ``window`` of them; one that sees nothing gets zeros. Tokens outside every sequence are
     not written.
 
-    ``max_q_len`` / ``max_kv_len``: the longest values the call may meet, if known (they
-    choose kernel and split; 0 stands for all tokens and the whole table). ``scale``
+    ``max_q_len`` / ``max_kv_len``: the longest values the call may meet, if known. They
+    choose kernel and split, and wrong ones cost time only; 0 stands for all tokens (without
+    ``q_starts``: for as many as each sequence has) and the whole table. A batch of single
+    or drafted tokens with ``q_starts`` and without ``max_q_len`` is taken for a prompt's
+    chunk, several times slower than need be. ``scale``
     defaults to ``head_dim ** -0.5``. Returns ``out`` like ``q`` (contiguous), with
     ``return_lse`` also the natural log-sum-exp of the scaled scores, float32
     ``[tokens, q_heads]``.
