@@ -39,6 +39,15 @@ Tensor bytes(size_t n, const at::Device& d) {
   return at::empty({static_cast<int64_t>(n)}, at::TensorOptions().dtype(at::kByte).device(d));
 }
 
+// The stride along axis i; an axis of one element may carry any, which does not count.
+int64_t stride_of(const Tensor& t, int64_t i) {
+  if (t.size(i) != 1) return t.stride(i);
+  return i + 1 < t.dim() ? t.size(i + 1) * stride_of(t, i + 1) : 1;
+}
+bool on_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// A copy, also of what is contiguous as it is but starts off a 16-byte boundary.
+Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+
 struct Cache {
   Tensor k, v;
   OptTensor k_scale, v_scale;
@@ -95,10 +104,9 @@ struct Cache {
                       " on the cache's device");
     TORCH_CHECK_VALUE(t.dim() == 3 && t.size(0) == tokens && t.size(1) == c.kv_heads && t.size(2) == c.head_dim, name,
                       " must be [tokens, num_kv_heads, head_dim]");
-    // rows of another layout (a transposed view) are copied once
-    const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    return fits ? t : t.contiguous();
+    // rows of another layout (a transposed view, a start off 16 bytes) are copied once
+    const bool fits = t.stride(2) == 1 && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 && on_16_bytes(t);
+    return fits ? t : copy_of(t);
   }
 
   void write(const Tensor& k_in, const Tensor& v_in, const Tensor& slots_in) const {
@@ -106,7 +114,7 @@ struct Cache {
     const int64_t n = slots.size(0);
     const OnDevice on(k.device());
     const Tensor a = rows_of(k_in, "k", n), b = rows_of(v_in, "v", n);
-    check(gemq_kv_cache_write(&c, a.data_ptr(), b.data_ptr(), a.stride(0), a.stride(1), b.stride(0), b.stride(1),
+    check(gemq_kv_cache_write(&c, a.data_ptr(), b.data_ptr(), stride_of(a, 0), stride_of(a, 1), stride_of(b, 0), stride_of(b, 1),
                               slots.data_ptr<int64_t>(), n, on.stream));
   }
 
@@ -144,9 +152,7 @@ std::pair<Tensor, OptTensor> attention(Tensor q, const Cache& cache, Tensor page
   const OnDevice on(dev);
   kv_lens = kv_lens.contiguous();
   if (page_table.stride(1) != 1) page_table = page_table.contiguous();
-  if (q.stride(2) != 1 || (q.stride(1) != q.size(2) && heads != 1) || q.stride(0) % 8 != 0 ||
-      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
-    q = q.contiguous();
+  if (q.stride(2) != 1 || stride_of(q, 1) != q.size(2) || stride_of(q, 0) % 8 != 0 || !on_16_bytes(q)) q = copy_of(q);
   Tensor out = at::empty({tokens, heads, q.size(2)}, q.options());
   OptTensor lse;
   if (return_lse) lse = at::empty({tokens, heads}, q.options().dtype(at::kFloat));
@@ -157,7 +163,7 @@ std::pair<Tensor, OptTensor> attention(Tensor q, const Cache& cache, Tensor page
   const size_t need = gemq_paged_attention_workspace_size(&cache.c, tokens, h, s, p, mq, mk);
   const Tensor ws = bytes(need, dev);
   const float factor = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
-  check(gemq_paged_attention(&cache.c, q.data_ptr(), q.stride(0), tokens, h, page_table.data_ptr<int32_t>(),
+  check(gemq_paged_attention(&cache.c, q.data_ptr(), stride_of(q, 0), tokens, h, page_table.data_ptr<int32_t>(),
                              page_table.stride(0), p, kv_lens.data_ptr<int32_t>(),
                              q_starts ? q_starts->data_ptr<int32_t>() : nullptr, s, mq, mk, factor,
                              static_cast<int32_t>(window), out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,

@@ -34,3 +34,35 @@ def test_without_starts_a_batch_of_few_tokens_takes_its_own_kernel(bits, each, m
     got = paged_attention(b.q, b.cache, b.page_table, b.kv_lens, max_q_len=max_q_len)
     assert torch.equal(got, want)
     b.check(use_starts=False, max_q_len=max_q_len)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("n", [1, 50])
+def test_queries_and_rows_that_start_off_16_bytes(bits, n):
+    """Contiguous tensors that begin anywhere in a buffer, and one token with a row stride
+    that is no multiple of 8."""
+    from robustgemq_b200.serving import paged_attention
+
+    b = Batch([(n, 90)], 4, 2, 64, 16, bits, H16)
+    want, _ = b.check()
+    for off in (1, 3, 8):
+        buf = torch.zeros(b.q.numel() + 16, dtype=H16, device="cuda")
+        q = buf[off:off + b.q.numel()].view_as(b.q)
+        q.copy_(b.q)
+        assert q.is_contiguous()
+        assert torch.equal(paged_attention(q, b.cache, b.page_table, b.kv_lens), want)
+        k = torch.randn((n, 2, 64), device="cuda").half()
+        rows = buf[off:off + k.numel()].view_as(k)
+        rows.copy_(k)
+        slots = b.slots(0, torch.arange(n, device="cuda"))
+        b.cache.write(k, k, slots)
+        first = b.cache.read(slots)
+        b.cache.write(torch.zeros_like(k), torch.zeros_like(k), slots)
+        b.cache.write(rows, rows, slots)
+        assert all(torch.equal(x, y) for x, y in zip(b.cache.read(slots), first))
+        b = Batch([(n, 90)], 4, 2, 64, 16, bits, H16)
+    if n == 1:
+        wide = torch.zeros((1, 4 * 64 + 3), dtype=H16, device="cuda")
+        wide[:, :256] = b.q.view(1, 256)
+        q = wide.as_strided((1, 4, 64), (259, 64, 1))
+        assert torch.equal(paged_attention(q, b.cache, b.page_table, b.kv_lens), want)
