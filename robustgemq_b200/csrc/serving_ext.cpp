@@ -44,6 +44,11 @@ int64_t stride_of(const Tensor& t, int64_t i) {
   if (t.size(i) != 1) return t.stride(i);
   return i + 1 < t.dim() ? t.size(i + 1) * stride_of(t, i + 1) : 1;
 }
+bool same_strides(const Tensor& a, const Tensor& b) {
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (stride_of(a, i) != stride_of(b, i)) return false;
+  return true;
+}
 bool on_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 // A copy, also of what is contiguous as it is but starts off a 16-byte boundary.
 Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
@@ -57,7 +62,7 @@ struct Cache {
   Cache(Tensor k_, Tensor v_, OptTensor ks, OptTensor vs, at::ScalarType dtype_)
       : k(std::move(k_)), v(std::move(v_)), k_scale(std::move(ks)), v_scale(std::move(vs)), dtype(dtype_) {
     TORCH_CHECK_VALUE(k.is_cuda(), "k must be a CUDA tensor (no CPU path)");
-    TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides() &&
+    TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && same_strides(v, k) &&
                           v.scalar_type() == k.scalar_type() && v.device() == k.device(),
                       "k and v must be alike: [num_pages, num_kv_heads, page_size, head_dim] on one device");
     TORCH_CHECK_VALUE(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be float16 or bfloat16");
@@ -73,20 +78,20 @@ struct Cache {
       const Tensor &a = *k_scale, &b = *v_scale;
       bool ok = a.dim() == (c.bits == 8 ? 3 : 4) && a.sizes().slice(0, 3) == k.sizes().slice(0, 3) &&
                 (c.bits == 8 || a.size(3) == 2);
-      ok = ok && b.sizes() == a.sizes() && b.strides() == a.strides() && a.scalar_type() == at::kFloat &&
+      ok = ok && b.sizes() == a.sizes() && same_strides(b, a) && a.scalar_type() == at::kFloat &&
            b.scalar_type() == at::kFloat && a.device() == k.device() && b.device() == k.device();
       TORCH_CHECK_VALUE(ok, "k_scale and v_scale must be float32 [num_pages, num_kv_heads, page_size] (4 bits: [..., 2]) "
                             "with the same strides, beside k");
       TORCH_CHECK_VALUE(c.bits == 8 || a.stride(3) == 1, "a row's step and base must be neighbours");
       c.k_scale = a.data_ptr<float>();
       c.v_scale = b.data_ptr<float>();
-      for (int i = 0; i < 3; ++i) c.scale_strides[i] = a.stride(i);
+      for (int i = 0; i < 3; ++i) c.scale_strides[i] = stride_of(a, i);
     }
     TORCH_CHECK_VALUE(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX && k.size(3) < INT32_MAX / 2,
                       "sizes must be below 2^31");
     c.k = k.data_ptr();
     c.v = v.data_ptr();
-    for (int i = 0; i < 3; ++i) c.strides[i] = k.stride(i) * static_cast<int64_t>(k.element_size());
+    for (int i = 0; i < 3; ++i) c.strides[i] = stride_of(k, i) * static_cast<int64_t>(k.element_size());
     c.num_pages = static_cast<int32_t>(k.size(0));
     c.kv_heads = static_cast<int32_t>(k.size(1));
     c.page_size = static_cast<int32_t>(k.size(2));

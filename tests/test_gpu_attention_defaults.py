@@ -66,3 +66,20 @@ def test_queries_and_rows_that_start_off_16_bytes(bits, n):
         wide[:, :256] = b.q.view(1, 256)
         q = wide.as_strided((1, 4, 64), (259, 64, 1))
         assert torch.equal(paged_attention(q, b.cache, b.page_table, b.kv_lens), want)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_caches_whose_axes_of_one_element_have_other_strides(bits):
+    """One page, K from a pool and V of its own: the strides between pages say nothing."""
+    from robustgemq_b200.serving import PagedKVCache
+
+    own = PagedKVCache(1, 16, 2, 64, bits=bits)
+    pool = torch.zeros((1, 3, *own.k.shape[1:]), dtype=own.k.dtype, device="cuda")
+    scales = () if bits == 16 else (torch.zeros((1, 5, *own.k_scale.shape[1:]), device="cuda")[:, 2], own.v_scale)
+    cache = PagedKVCache.from_tensors(pool[:, 1], own.v, *scales, dtype=H16)
+    x, y = (torch.randn((16, 2, 64), device="cuda").half() for _ in range(2))
+    slots = torch.arange(16, device="cuda")
+    cache.write(x, y, slots)
+    own.write(x, y, slots)
+    for got, want in zip(cache.read(slots), own.read(slots)):
+        assert torch.equal(got, want)
