@@ -26,6 +26,7 @@
 // bytes, the rest the exponentials' pipe and the uneven last round; 24 of up to 5, 32,001
 // fp32 (rows off 16-byte boundaries, so single loads): 12.8 us, latency.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged.cuh"
 
@@ -206,8 +207,9 @@ __device__ __forceinline__ Stat row_stat(const L* row, int j, int j1, int stride
   return greedy ? row_stat<false, true>(row, j, j1, stride, f) : row_stat<false, false>(row, j, j1, stride, f);
 }
 
-// log2(e) / T; the greedy form keeps T = 1 for its log probabilities.
-__device__ __forceinline__ float slope(float t) { return kLog2e / (t == 0.f ? 1.f : t); }
+// log2(e) / T; the greedy form keeps T = 1 for its log probabilities. Of a subnormal T the
+// quotient is infinite, and times the maximum's distance from itself it would be a NaN.
+__device__ __forceinline__ float slope(float t) { return fminf(kLog2e / (t == 0.f ? 1.f : t), FLT_MAX); }
 
 template <typename L>
 __global__ void __launch_bounds__(kThreads, kStatBlocks) k_verify_stats(const VerifyArgs a) {
