@@ -195,7 +195,7 @@ def load(build_if_stale: bool = True) -> ctypes.CDLL:
         if build_if_stale:
             from . import build as _build
             try:
-                _build.build()
+                _build.build_library()
             except Exception as exc:  # no nvcc on this machine: fall through to a prebuilt .so
                 if not LIB_PATH.exists():
                     raise RuntimeError(f"libgemq_b200.so is missing and could not be built: {exc}") from exc

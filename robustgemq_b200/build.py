@@ -72,22 +72,51 @@ def _ext_commands(obj: Path):
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
-    """Builds the library and, beside it, the torch binding of the serving operators."""
-    ext = None
+    """Builds the library and, beside it, the torch binding of the serving operators. The
+    library does not need the binding: it is built before what stops that is raised."""
+    ext, failed = None, None
     if force or _ext_stale():
-        objdir = ROOT / "_build"
-        objdir.mkdir(exist_ok=True)
-        compile_cmd, link_cmd = _ext_commands(objdir / "serving_ext.o")
-        ext = subprocess.Popen(compile_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        try:
+            ext = _start_ext()
+        except Exception as exc:  # no g++, no Python headers
+            failed = exc
+    build_library(force, verbose, jobs)
+    if failed is not None:
+        raise RuntimeError(f"the torch binding could not be built: {failed}") from failed
+    if ext is not None:
+        _finish_ext(ext, verbose)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
+    """Builds the library where its sources are newer."""
     if force or _stale():
         _build_lib(verbose, jobs)
-    if ext is not None:
-        _wait((EXT_SOURCE, ext), verbose)
-        out = subprocess.run(link_cmd, capture_output=True, text=True)
-        if out.returncode != 0:
-            raise RuntimeError(f"link failed:\n{out.stdout}\n{out.stderr}")
-        os.replace(EXT.with_suffix(".so.tmp"), EXT)
     return LIB
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """Builds the torch binding (beside a library that is there) where its sources are
+    newer."""
+    if _ext_stale():
+        _finish_ext(_start_ext(), verbose)
+    return EXT
+
+
+def _start_ext():
+    objdir = ROOT / "_build"
+    objdir.mkdir(exist_ok=True)
+    compile_cmd, link_cmd = _ext_commands(objdir / "serving_ext.o")
+    return subprocess.Popen(compile_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True), link_cmd
+
+
+def _finish_ext(ext, verbose: bool) -> None:
+    proc, link_cmd = ext
+    _wait((EXT_SOURCE, proc), verbose)
+    out = subprocess.run(link_cmd, capture_output=True, text=True)
+    if out.returncode != 0:
+        raise RuntimeError(f"link failed:\n{out.stdout}\n{out.stderr}")
+    os.replace(EXT.with_suffix(".so.tmp"), EXT)
 
 
 def _build_lib(verbose: bool, jobs: int) -> Path:

@@ -22,8 +22,10 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from . import build as _build
 
-_lib.load()  # builds the library and its torch binding first if their sources are newer
+_lib.load()
+_build.build_binding()  # where its sources are newer
 from . import _serving_ext as _ext  # noqa: E402
 
 
