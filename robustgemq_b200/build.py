@@ -26,6 +26,7 @@ SOURCES = ["gemq_api.cu", "kernels_misc.cu", "kernels_route.cu", "kernels_decode
 # the torch binding of the serving operators
 EXT = PKG / "_serving_ext.so"
 EXT_SOURCE = "serving_ext.cpp"
+EXT_STAMP = ROOT / "_build" / "serving_ext.torch"  # the torch version it was compiled with
 HEADERS = ["gemq_common.cuh", "gemq_internal.h", "tc_work.cuh", "kperm.cuh", "paged.cuh", "attn_rows.cuh"]
 # compiled without relocatable device code: ptxas ignores setmaxnreg with it
 WHOLE = {"kernels_attn_tc.cu"}
@@ -50,8 +51,16 @@ def _stale() -> bool:
 def _ext_stale() -> bool:
     if not EXT.exists():
         return True
+    if EXT_STAMP.exists() and EXT_STAMP.read_text() != _torch_version():
+        return True  # another torch's headers
     t = EXT.stat().st_mtime
     return any(p.stat().st_mtime > t for p in (CSRC / EXT_SOURCE, ROOT / "include" / "gemq_b200.h"))
+
+
+def _torch_version() -> str:
+    import torch
+
+    return torch.__version__
 
 
 def _ext_commands(obj: Path):
@@ -97,7 +106,7 @@ def build_library(force: bool = False, verbose: bool = False, jobs: int = 4) -> 
 
 def build_binding(verbose: bool = False) -> Path:
     """Builds the torch binding (beside a library that is there) where its sources are
-    newer."""
+    newer or torch is another."""
     if _ext_stale():
         _finish_ext(_start_ext(), verbose)
     return EXT
@@ -117,6 +126,7 @@ def _finish_ext(ext, verbose: bool) -> None:
     if out.returncode != 0:
         raise RuntimeError(f"link failed:\n{out.stdout}\n{out.stderr}")
     os.replace(EXT.with_suffix(".so.tmp"), EXT)
+    EXT_STAMP.write_text(_torch_version())
 
 
 def _build_lib(verbose: bool, jobs: int) -> Path:

@@ -32,3 +32,16 @@ def test_loading_the_library_leaves_the_binding_alone(monkeypatch, made):
     monkeypatch.setattr(_lib, "_lib", None)
     lib = _lib.load()
     assert made == ["library"] and lib.gemq_version() == (whole or lib).gemq_version()
+
+
+def test_a_binding_of_another_torch_is_stale(monkeypatch, tmp_path):
+    ext = tmp_path / "ext.so"
+    ext.write_bytes(b"")
+    stamp = tmp_path / "stamp"
+    monkeypatch.setattr(build, "EXT", ext)
+    monkeypatch.setattr(build, "EXT_STAMP", stamp)
+    assert not build._ext_stale()  # a binding without a stamp goes by its sources
+    stamp.write_text(build._torch_version())
+    assert not build._ext_stale()
+    stamp.write_text("0.0.1")
+    assert build._ext_stale()
