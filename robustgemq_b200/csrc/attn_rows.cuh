@@ -1,32 +1,22 @@
-// One attention row by one block, in fp32 on the CUDA cores: the plainest form, which the
-// tensor-core kernel falls back on for rows its tiles cannot keep apart.
+// One attention row by one block over a cache of 16 bits, in fp32 on the CUDA cores: the
+// plainest form, which the kernel for chunks falls back on for rows its tiles cannot keep
+// apart (codes need no such form: a key's factors say what is no number).
 #pragma once
 
 #include "paged.cuh"
 
 namespace gemq {
 
-// Eight elements of a stored row, from element 8 * c.
-template <typename T, int BITS>
-__device__ __forceinline__ void load8(const uint8_t* row, int c, float step, float base, float (&x)[8]) {
-  if constexpr (BITS == 16) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + c * 16);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// Eight elements of a row, from element 8 * c.
+template <typename T>
+__device__ __forceinline__ void load8(const uint8_t* row, int c, float (&x)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(row + c * 16);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2<T>(u[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  } else if constexpr (BITS == 8) {
-    const uint2 w = *reinterpret_cast<const uint2*>(row + c * 8);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)))) * step;
-  } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + c * 4);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((w >> (4 * i)) & 15u), step, base);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(u[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
   }
 }
 
@@ -57,7 +47,7 @@ __device__ __forceinline__ float row_reduce(float v, bool is_max, float* red) {
 // One row by one block of kAttnRowThreads threads, in fp32 throughout: a thread takes whole
 // keys for the scores and then elements of the output. Keys that the row does not see
 // are never read.
-template <typename T, int BITS>
+template <typename T>
 __device__ void attn_one_row(const AttnArgs& a, int b, const SeqRange& r, int i, int h, AttnRowSmem& sm) {
   const int D = a.kv.head_dim;
   const int kvh = h / a.group;
@@ -77,16 +67,10 @@ __device__ void attn_one_row(const AttnArgs& a, int b, const SeqRange& r, int i,
       const int page = page_of(a, b, j >> a.kv.page_shift);
       if (page >= 0) {
         const uint8_t* row = a.kv.k + a.kv.row(page, kvh, j & mask);
-        float step = 1.f, base = 0.f;
-        if constexpr (BITS != 16) {
-          const float* sc = a.kv.k_scale + a.kv.scale_row(page, kvh, j & mask);
-          step = sc[0];
-          if constexpr (BITS == 4) base = sc[1];
-        }
         float dot = 0.f;
         for (int c = 0; c < D / 8; ++c) {
           float x[8];
-          load8<T, BITS>(row, c, step, base, x);
+          load8<T>(row, c, x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) dot = fmaf(sm.q[8 * c + e], x[e], dot);
         }
@@ -112,15 +96,7 @@ __device__ void attn_one_row(const AttnArgs& a, int b, const SeqRange& r, int i,
         const int page = page_of(a, b, jj >> a.kv.page_shift);
         if (page < 0) continue;
         const uint8_t* row = a.kv.v + a.kv.row(page, kvh, jj & mask);
-        float x;
-        if constexpr (BITS == 16) {
-          x = to_f32(reinterpret_cast<const T*>(row)[d]);
-        } else {
-          const float* sc = a.kv.v_scale + a.kv.scale_row(page, kvh, jj & mask);
-          if constexpr (BITS == 8) x = static_cast<float>(reinterpret_cast<const int8_t*>(row)[d]) * sc[0];
-          else x = fmaf(static_cast<float>((row[d >> 1] >> (4 * (d & 1))) & 15), sc[0], sc[1]);
-        }
-        acc = fmaf(sm.p[t], x, acc);
+        acc = fmaf(sm.p[t], to_f32(reinterpret_cast<const T*>(row)[d]), acc);
       }
       o[u] = acc;
     }

@@ -37,7 +37,6 @@
 // heads, fp16: 9.9 us, 1.7 TB/s, latency (page table, keys, join in turn).
 #include <algorithm>
 
-#include "attn_rows.cuh"
 #include "paged.cuh"
 
 namespace gemq {

@@ -1037,7 +1037,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attn_tiles(const AttnArgs a, c
       const TileNote note = ta.note[first_block(item)];
       const SeqRange r = seq_range(a, note.seq);
       for (int row = 0; row < note.rows; ++row)
-        attn_one_row<T, BITS>(a, note.seq, r, (note.row0 + row) / a.group, note.head * a.group + (note.row0 + row) % a.group, sm);
+        attn_one_row<T>(a, note.seq, r, (note.row0 + row) / a.group, note.head * a.group + (note.row0 + row) % a.group, sm);
     }
   }
 }
