@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, BITS, DP, NR>::kBlocks) k_att
           vstep = vv.x;
           vbase = fmaf(8.f, vv.x, vv.y);
         }
-        vstep = vstep < kMinScale ? kMinScale : vstep;  // a step of zero; a NaN stays
+        vstep = value_step(vstep, vbase);
         const float lv = lg2(vstep);
         prep[lane] = step * cs * kUp;
         prep[kKeys + lane] = lv;

@@ -678,11 +678,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_many(const AttnArgs a, con
         // that see the key and no others; the rest must then be numbers.
         if (me < kKeys) {
           float* const prep = s_prep + (t & 1) * (K::kPrepTile / 4);
-          const float vs = vstep.x < kMinScale ? kMinScale : vstep.x;  // a step of zero; a NaN stays
+          const float vbase = BITS == 4 ? fmaf(8.f, vstep.x, vstep.y) : 0.f;
+          const float vs = value_step(vstep.x, vbase);
           const float lv = lg2(vs);
           bool bad = !(vs < INFINITY);
           if constexpr (BITS == 4) {
-            const float zr = fmaf(8.f, vstep.x, vstep.y) / vs;
+            const float zr = vbase / vs;
             bad = bad || !(fabsf(zr) < INFINITY);
             prep[3 * kKeys + me] = fmaf(8.f, kstep.x, kstep.y) * cs;
             prep[4 * kKeys + me] = bad ? 0.f : zr;

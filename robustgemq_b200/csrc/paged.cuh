@@ -18,6 +18,15 @@ namespace gemq {
 // times any sequence length inside fp32.
 constexpr float kMinScale = 5.421010862427522e-20f;  // 2^-64
 
+// The step t with which a value row counts in attention, `base` its offset (the value of
+// code 8 at 4 bits): what is stored, but at least 2^-64 (a step of zero) and 2^-100 |base|,
+// so that base / t stays in fp32 for a row of large equal values, whose codes say nothing.
+// Either moves a value by less than 2^-96 of it. A NaN stays.
+__device__ __forceinline__ float value_step(float stored, float base) {
+  const float least = fmaxf(kMinScale, fabsf(base) * 7.888609052210118e-31f);
+  return stored < least ? least : stored;
+}
+
 // gemq_kv_cache_t as the kernels take it. Strides between pages, heads and tokens: of the
 // codes in units of 8 bytes, of the scales in floats; below 2^31 each, so that a row's
 // address takes three 32 x 32 -> 64 bit multiply-adds.

@@ -136,3 +136,27 @@ def test_loud_values_without_weight(bits, dtype, heads, kv_heads, dim, n, length
     b = make(n, length, heads, kv_heads, dim, bits, dtype, loud, GAIN[H16], k_of)
     b.q[..., 0] = 4.0
     check_rows(b, 0)
+
+
+def large_equal(bits, heads, kv_heads, dim, n, length, size):
+    """A batch, its keys and bf16 value rows of one large value each."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    b = Batch([(n, length), (3, 40)], heads, kv_heads, dim, 16, bits, B16, seed=dim + n)
+    k = torch.randn((length, kv_heads, dim), generator=gen, device="cuda").to(B16)
+    v = (torch.rand((length, kv_heads, 1), generator=gen, device="cuda") * 2 - 1) * size
+    return b, k, v.expand(length, kv_heads, dim).to(B16).contiguous()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("n,length", [(3, 200), (60, 400), (300, 700)])
+@pytest.mark.parametrize("size", [1e12, 1e20, 1e30, 1e38])
+def test_rows_of_large_equal_values_at_4_bits(heads, kv_heads, dim, n, length, size):
+    """Rows whose step is 2^-64, with all of the value in the base: alone, and between rows of
+    zeros."""
+    b, k, v = large_equal(4, heads, kv_heads, dim, n, length, size)
+    at = torch.arange(length, device="cuda")
+    replace(b, 0, at, k, v)
+    check_rows(b, 0)
+    v[::2] = 0.0
+    replace(b, 0, at, k, v)
+    check_rows(b, 0)
