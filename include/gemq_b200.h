@@ -402,7 +402,8 @@ int gemq_kv_cache_read(const gemq_kv_cache_t* cache /* host */, const int64_t* s
  * page_table[b * page_table_stride + j / page_size]. Token i of n sees the positions
  * j <= kv_lens[b] - n + i, and with window > 0 only the last `window` of those; a row
  * that sees nothing gives zeros and lse -inf, and what a row does not see does not reach
- * it, whatever it holds. q_heads is a multiple of kv_heads; head h reads KV head
+ * it, whatever it holds (at 8 and 4 bits a value row with a step above 2^38 counts as one
+ * with a NaN, in the rows that see it). q_heads is a multiple of kv_heads; head h reads KV head
  * h / (q_heads / kv_heads). q [num_tokens, q_heads, head_dim] (token stride in elements,
  * a multiple of 8; 16-byte aligned); out the same, contiguous; lse fp32 [num_tokens,
  * q_heads] or NULL: the natural logarithm of the sum of exp(scale * score). Scores,

@@ -21,10 +21,15 @@ constexpr float kMinScale = 5.421010862427522e-20f;  // 2^-64
 // The step t with which a value row counts in attention, `base` its offset (the value of
 // code 8 at 4 bits): what is stored, but at least 2^-64 (a step of zero) and 2^-100 |base|,
 // so that base / t stays in fp32 for a row of large equal values, whose codes say nothing.
-// Either moves a value by less than 2^-96 of it. A NaN stays.
+// Either moves a value by less than 2^-96 of it. A NaN stays. A step above 2^38 (only bf16
+// rows of values above 10^12 have one) is none: a weight is held as 2^x t beside the largest
+// one that the row sees, and where steps reach from 2^-64 (rows of zeros) further than that,
+// keys of equal weight fall out of fp32 and were lost from the sum of the weights.
+constexpr float kMaxValueStep = 274877906944.f;  // 2^38
 __device__ __forceinline__ float value_step(float stored, float base) {
   const float least = fmaxf(kMinScale, fabsf(base) * 7.888609052210118e-31f);
-  return stored < least ? least : stored;
+  const float step = stored < least ? least : stored;
+  return step > kMaxValueStep ? NAN : step;
 }
 
 // gemq_kv_cache_t as the kernels take it. Strides between pages, heads and tokens: of the

@@ -160,3 +160,42 @@ def test_rows_of_large_equal_values_at_4_bits(heads, kv_heads, dim, n, length, s
     v[::2] = 0.0
     replace(b, 0, at, k, v)
     check_rows(b, 0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("n,length", [(3, 200), (60, 400), (300, 700)])
+@pytest.mark.parametrize("size", [1e12, 1e20, 1e30, 1e38])
+def test_rows_of_large_equal_values_at_8_bits(heads, kv_heads, dim, n, length, size):
+    """Between rows of zeros, whose step is 2^-64: the rows of zeros keep their weight, or,
+    where the steps lie too far apart for that, every row that sees a large value is NaN."""
+    from robustgemq_b200.serving import paged_attention
+
+    b, k, v = large_equal(8, heads, kv_heads, dim, n, length, size)
+    v = (v.float() / 127).to(B16)  # 127 times the largest has to stay in fp32
+    at = torch.arange(length, device="cuda")
+    v[::2] = 0.0
+    replace(b, 0, at, k, v)
+    if size / 127 / 127 < 2.0 ** 38:
+        check_rows(b, 0)
+    else:
+        out = paged_attention(b.q, b.cache, b.page_table, b.kv_lens, q_starts=b.q_starts)
+        assert torch.isnan(out[:n]).all()
+        check_rows(b, 1)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("n,length", [(3, 200), (60, 400), (300, 700)])
+def test_steps_that_are_none_stay_with_the_rows_that_see_them(bits, heads, kv_heads, dim, n, length):
+    """A value row of 1e30 in the chunk: NaN from its position on, nothing before it."""
+    from robustgemq_b200.serving import paged_attention
+
+    loud = length - (n + 2) // 3
+    b = make(n, length, heads, kv_heads, dim, bits, B16, torch.tensor([], dtype=torch.int64), 1.0)
+    want = paged_attention(b.q, b.cache, b.page_table, b.kv_lens, q_starts=b.q_starts)
+    v = torch.randn((1, kv_heads, dim), device="cuda").mul_(1e30).to(B16)
+    b.put(0, torch.tensor([loud], device="cuda"), torch.zeros_like(v), v)
+    out = paged_attention(b.q, b.cache, b.page_table, b.kv_lens, q_starts=b.q_starts)
+    first = loud - (length - n)
+    assert torch.equal(out[:first], want[:first]) and torch.equal(out[n:], want[n:])
+    assert torch.isnan(out[first:n]).all()
