@@ -95,7 +95,8 @@ KvDev to_dev(const gemq_kv_cache_t& c) {
 
 int check_rows(const gemq_kv_cache_t* c, int64_t tokens) {
   if (tokens < 0) return fail(GEMQ_ERR_INVALID_ARGUMENT, "tokens must not be negative");
-  if (tokens * c->kv_heads > (int64_t{1} << 29)) return fail(GEMQ_ERR_UNSUPPORTED, "tokens * kv_heads above 2^29");
+  if (tokens > (int64_t{1} << 29) || tokens * c->kv_heads > (int64_t{1} << 29))
+    return fail(GEMQ_ERR_UNSUPPORTED, "tokens * kv_heads above 2^29");
   return GEMQ_OK;
 }
 
@@ -107,7 +108,7 @@ int check_attention(const gemq_kv_cache_t* c, int64_t num_tokens, int32_t q_head
     return fail(GEMQ_ERR_INVALID_ARGUMENT, "negative size");
   if (q_heads % c->kv_heads != 0)
     return fail(GEMQ_ERR_INVALID_ARGUMENT, "q_heads must be a multiple of the cache's kv_heads");
-  if (num_tokens * q_heads > (int64_t{1} << 29) || num_seqs > (1 << 20))
+  if (num_tokens > (int64_t{1} << 29) || num_tokens * q_heads > (int64_t{1} << 29) || num_seqs > (1 << 20))
     return fail(GEMQ_ERR_UNSUPPORTED, "num_tokens * q_heads above 2^29, or more than 2^20 sequences");
   if (static_cast<int64_t>(max_pages) * c->page_size > INT32_MAX)
     return fail(GEMQ_ERR_UNSUPPORTED, "max_pages * page_size must be below 2^31");
