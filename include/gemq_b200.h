@@ -383,7 +383,7 @@ typedef struct gemq_kv_cache {
 /* Writes token t's keys and values k, v [tokens, kv_heads, head_dim] (strides in elements
  * between tokens and heads; rows 16-byte aligned) to slot slots[t]. A negative slot skips
  * its token, one past the cache is recorded in the device error word and skipped; of two
- * tokens with one slot either may stay. Per row x: 8 bits m = max(max|x|, 127 * 2^-64),
+ * tokens with one slot parts of both may stay, so give a slot once. Per row x: 8 bits m = max(max|x|, 127 * 2^-64),
  * code rint(127 x / m), step m / 127; 4 bits lo = min x, r = max(max x - lo, 15 * 2^-64),
  * code rint(15 (x - lo) / r), step r / 15, base lo. A row with a NaN, an infinity or a
  * product above that leaves fp32 reads back as NaN throughout. */
@@ -426,7 +426,7 @@ int gemq_paged_attention(const gemq_kv_cache_t* cache /* host */, const void* q,
 /* Verification of drafted tokens. p_i = softmax(logits[b][i] / temperature[b]) (NULL: 1;
  * 0: all of it on the first maximum); draft i < draft_lens[b] (NULL: num_drafts) is taken
  * while uniforms[b][i] * q_i(x_i) < p_i(x_i), with q_i = draft_probs[b][i] (NULL: the
- * draft was certain, q_i(x_i) = 1). At the first position r that is not taken, or at the
+ * draft was certain, q_i(x_i) = 1); a length outside [0, num_drafts] is clamped. At the first position r that is not taken, or at the
  * draft's end, one token is drawn from w = max(p_r - q_r, 0) (at the end, or where that
  * leaves nothing, w = p_r): the j with the largest w_j / noise[b][j], lowest j on ties;
  * exponential noise makes that a sample of w / sum(w).

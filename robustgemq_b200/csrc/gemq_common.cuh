@@ -197,16 +197,21 @@ __device__ __forceinline__ bool mbar_wait_drain(uint64_t* bar, uint32_t parity) 
 // The decode-path kernels are launched with programmatic stream serialization and
 // call grid_dep_wait() before they touch any global buffer; the wait returns once the
 // previous kernel in the stream has finished and its writes are visible (at once when
-// launched without the attribute). No kernel triggers its dependents early: measured
-// on B200, letting the next kernel become resident before this one finished slowed
-// the decode stack by 5-10% (early kernels hold shared memory on SMs that a
-// one-CTA-per-SM kernel behind them needs), while launching at completion through the
-// programmatic edge gains about 1% over plain stream order.
+// launched without the attribute). The kernels of a layer's forward do not trigger their
+// dependents early, but for the pairs named below: measured on B200, letting the next
+// kernel become resident before this one finished slowed the decode stack by 5-10% (early
+// kernels hold shared memory on SMs that a one-CTA-per-SM kernel behind them needs), while
+// launching at completion through the programmatic edge gains about 1% over plain stream
+// order.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// The one exception: the gate/up GEMM of a layer forward lets its down-projection
-// GEMM be scheduled (onto SMs its own CTAs have left) once each of its CTAs has begun
-// its last item; the down GEMM then waits per token tile on counters instead of on
-// grid completion (tile_done_signal / tile_done_wait).
+// Lets the next kernel come up before this one has ended, once each CTA has called it. In
+// a layer's forward the gate/up GEMM lets its down-projection GEMM be scheduled (onto SMs
+// its own CTAs have left) once each of its CTAs has begun its last item, and the gate/up
+// GEMV its down GEMV; the down kernel then waits per token tile on counters instead of on
+// grid completion (tile_done_signal / tile_done_wait). The serving operators' first
+// kernels (the cache's write and read, attention of few rows, the verification's
+// statistics) call it after their own wait: whatever comes next waits for the whole grid
+// before it touches what that grid writes.
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Counter handshake between CTAs of two kernels. The producer: every lane stores its

@@ -31,10 +31,12 @@
 // were cut.
 //
 // Measured on a B200: 2 sequences of 131,072, 32 query and 8 KV heads x 128, bf16: 164 us,
-// 6.5 TB/s, bytes. 64 uneven ones up to 8,192, 32 on 4 heads, 8 bits: 61.5 us, 4.6 TB/s;
-// 16 up to 4,096, 5 tokens each, 16 heads, 4 bits: 39.3 us, 2.2 TB/s: both issue slots,
-// unpacking and factors, the second a third of it a piece's set-up and join. 1 of 2,048, 16
-// heads, fp16: 9.9 us, 1.7 TB/s, latency (page table, keys, join in turn).
+// 6.5 TB/s, bytes. 64 uneven ones up to 8,192, 32 on 4 heads, 8 bits: 62 us, 4.6 TB/s, and
+// 16 up to 4,096, 5 tokens each, 16 heads, 4 bits: 39.5 us, 2.2 TB/s: neither bytes (57% and
+// 28% of the DRAM's time) nor issue slots (58% and 55%) are used up; a scheduler has two or
+// three warps, each a chain of unpacking, product, maximum, exponentials and product, and
+// the second spends a third of its time on pieces' set-up and join. 1 of 2,048, 16 heads,
+// fp16: 9.8 us, 1.7 TB/s, latency (page table, keys, join in turn).
 #include <algorithm>
 
 #include "paged.cuh"

@@ -40,11 +40,13 @@
 // at 8 and 4 bits, the loaders' unpacking, against 2,810 and 1,683.)
 //
 // Measured on a B200: 4,096 tokens at the end of 16,384, 32 query and 8 KV heads x 128,
-// bf16: 890 us (1,080 TFLOP/s of the visible pairs; 1,020 us in long runs under the power
-// limit), the exponentials' pipe and the softmax warps' issue. 12 uneven chunks up to 1,000
-// of 9,000, 24 on 8 heads x 64, window 4,096, 8 bits: 480 us (327 TFLOP/s), the softmax
-// warps' chain of waits, factors and exponentials, which half as many columns leave twice as
-// often.
+// bf16: 900 us (1,070 TFLOP/s of the visible pairs; 1,030 us in long runs under the power
+// limit), with the exponentials' pipe and the tensor cores half used each and 47% of the
+// issue slots: two softmax warps a scheduler do not cover each other's waits. At 8 and 4
+// bits 2,090 and 2,440 us, the loaders' unpacking and the factors. 12 uneven chunks up to
+// 1,000 of 9,000, 24 on 8 heads x 64, window 4,096, 8 bits: 477 us (330 TFLOP/s), issue 42%,
+// shared memory 38%, the exponentials' pipe 36% used: the softmax warps' chain of waits,
+// factors, maximum and exponentials.
 #define GEMQ_OWN_ERROR_WORDS  // compiled without relocatable device code, for setmaxnreg
 #include <cudaTypedefs.h>
 

@@ -9,11 +9,15 @@
 // A row with a NaN, an infinity, or a range whose product above leaves fp32 stores NaN
 // as its step and reads back as NaN throughout: the damage stays in that token and head.
 //
-// Each pass reads its rows once and writes them once, so bytes bound it: measured on a
-// B200, written and read back, 50,001 tokens of 8 heads x 80, 8 bits: 81 us for 391 MB
-// (4.8 TB/s of the copy's 6.65; the read is at 6.0, the write is held by its instructions
-// as much as by bytes); 8,192 of 4 x 128, 4 bits: 15 us for 43 MB, two launches
-// that each last a few memory latencies; 64 of 16 x 128: 4 us, one latency each.
+// Of two tokens written to one slot parts of both may stay: a row's pieces and its scale are
+// separate stores of separate warps.
+//
+// Each pass reads its rows once and writes them once. Measured on a B200, written and read
+// back in one graph, 50,001 tokens of 8 heads x 80, 8 bits: 81 us for 391 MB (4.8 TB/s of
+// the copy's 6.56; the read is at 6.0; the write takes 54 for 30 us of bytes, a warp's loads,
+// reductions and stores one after the other and 68% of its issue slots used); 8,192 of
+// 4 x 128, 4 bits: 15 us for 43 MB, two launches that each last a few memory latencies; 64
+// of 16 x 128: 4 us, one latency each.
 //
 // Multiplying before the one division (both products are exact for 16-bit inputs whose
 // differences fit fp32) makes the halves that the rounding meets exact halves, so a code

@@ -23,8 +23,9 @@
 // Measured on a B200, with the bytes that must move against the copy bandwidth: 1
 // sequence of 4 drafts, vocabulary 50,304, fp16: 8.3 us, latency (two launches, four
 // dependent reads); 64 of 7, 151,936, bf16 with fp32 probabilities: 54.2 us, 35.5 of
-// bytes, the rest the exponentials' pipe and the uneven last round; 24 of up to 5, 32,001
-// fp32 (rows off 16-byte boundaries, so single loads): 12.8 us, latency.
+// bytes: the statistics use the exponentials' pipe to 65% and the DRAM to half, the pick
+// waits for its loads, a step at a time (30% of the issue slots); 24 of up to 5, 32,001
+// fp32 (rows off 16-byte boundaries, so single loads): 12.5 us, latency.
 #include <algorithm>
 #include <cfloat>
 

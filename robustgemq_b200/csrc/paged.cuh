@@ -212,7 +212,7 @@ cudaError_t launch_cache_read(const KvDev& c, int bits, bool bf16, const int64_t
 size_t attention_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len);
 cudaError_t launch_attention(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
                              cudaStream_t s);
-// (kernels_attn_tc.cu: many rows a KV head; head_dim at most 128)
+// (kernels_attn_tc.cu: many rows a KV head)
 size_t many_workspace(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len);
 cudaError_t launch_many(const AttnArgs& a, int bits, bool bf16, int max_q_len, int max_kv_len, void* workspace,
                         cudaStream_t s);

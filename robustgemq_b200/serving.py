@@ -74,8 +74,10 @@ class PagedKVCache(_ext.Cache):
 
     def write(self, k: Tensor, v: Tensor, slots: Tensor) -> None:
         """Quantises token ``t``'s rows ``k[t]``, ``v[t]`` (``[tokens, num_kv_heads,
-        head_dim]``) into slot ``slots[t]`` (int64). A negative slot skips its token. A row
-        with a NaN or an infinity reads back as NaN throughout (8 and 4 bits)."""
+        head_dim]``) into slot ``slots[t]`` (int64). A negative slot skips its token; a slot
+        given twice is left with parts of both tokens. At 8 and 4 bits a row reads back as
+        NaN throughout where it has a NaN or an infinity, or where (bfloat16) 127 times its
+        largest magnitude, or 15 times its range, leaves float32."""
         super().write(k, v, slots)
 
     def read(self, slots: Tensor) -> Tuple[Tensor, Tensor]:
@@ -97,7 +99,8 @@ def paged_attention(q: Tensor, cache: PagedKVCache, page_table: Tensor, kv_lens:
     ``page_table[b, j // page_size]``. Query heads share KV heads in equal groups. Token
     ``i`` of ``n`` sees the positions up to ``kv_len - n + i``, with ``window > 0`` the last
     ``window`` of them; one that sees nothing gets zeros. Tokens outside every sequence are
-    not written.
+    not written. At 8 and 4 bits a value row whose step is above 2^38 (bfloat16 values
+    above 10^12) counts as NaN in the tokens that see it.
 
     ``max_q_len`` / ``max_kv_len``: the longest values the call may meet, if known. They
     choose kernel and split, and wrong ones cost time only; 0 stands for all tokens (without
@@ -130,7 +133,8 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
 
     ``target_logits [seqs, drafts + 1, vocab]`` (float16, bfloat16 or float32): the
     target's logits at the last known token and at every draft. ``draft_tokens`` int64
-    ``[seqs, drafts]``, ``draft_lens`` int32 ``[seqs]`` how many of them count (all).
+    ``[seqs, drafts]``, ``draft_lens`` int32 ``[seqs]`` how many of them count (all; clamped
+    to what there are).
     ``draft_probs [seqs, drafts, vocab]``: what the draft sampled from; left out for drafts
     made without sampling. ``temperature`` float32 ``[seqs]`` (1; 0: greedy). The random
     numbers are given: ``uniforms`` float32 ``[seqs, drafts]`` in [0, 1) and ``noise``
