@@ -36,8 +36,8 @@
 // same 128 rows and all keys, 64 at a time, and half of V's columns each. S and P are formed
 // twice, so two of six products are repeated, but Q and the keys stand in shared memory
 // once, and all else stays as it is. (2,048 tokens at the end of 8,192, 16 query and 4 KV
-// heads x 256: 334 us, 720 TFLOP/s, at 16 bits, where 16-row tiles took 3,141; 711 and 730
-// at 8 and 4 bits, the loaders' unpacking, against 2,810 and 1,683.)
+// heads x 256: 334 us, 720 TFLOP/s, at 16 bits, where 16-row tiles took 3,141; 711 to 759
+// and 730 to 745 at 8 and 4 bits, the loaders' unpacking, against 2,810 and 1,683.)
 //
 // Measured on a B200: 4,096 tokens at the end of 16,384, 32 query and 8 KV heads x 128,
 // bf16: 900 us (1,070 TFLOP/s of the visible pairs; 1,030 us in long runs under the power
